@@ -20,6 +20,7 @@ constexpr float kGateC = -8.0f;  // hawk/scan_fused.py:44,123
   } while (0)
 
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+__device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 inline bool valid_dtype(int d) { return d == HAWK_F32 || d == HAWK_BF16; }
 inline size_t dtype_size(int d) { return d == HAWK_BF16 ? 2 : 4; }
 inline int launch_status() { return cudaGetLastError() == cudaSuccess ? HAWK_OK : HAWK_ERR_LAUNCH; }

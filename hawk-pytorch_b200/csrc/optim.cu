@@ -33,7 +33,10 @@ struct AdamwTable {
   int count;
 };
 
-__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamwTable tab, AdamwArgs a) {
+// grad_scale: a device scalar times which the gradients are taken (the clip of a global norm: they are read here anyway, and
+// a pass of its own would read and write them once more, 8 of 36 bytes per element); null = 1
+__global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ AdamwTable tab, AdamwArgs a, const float* grad_scale) {
+  const float gs = grad_scale ? *grad_scale : 1.f;
   int lo = 0, hi = tab.count;  // the tensor whose blocks hold this one
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -55,10 +58,10 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
       float4 pv = reinterpret_cast<float4*>(p)[i];
       const float4 gv = __ldg(reinterpret_cast<const float4*>(g) + i);
       float4 mv = reinterpret_cast<float4*>(m)[i], vv = reinterpret_cast<float4*>(v)[i];
-      pv.x = adamw_one(pv.x, gv.x, mv.x, vv.x, a);
-      pv.y = adamw_one(pv.y, gv.y, mv.y, vv.y, a);
-      pv.z = adamw_one(pv.z, gv.z, mv.z, vv.z, a);
-      pv.w = adamw_one(pv.w, gv.w, mv.w, vv.w, a);
+      pv.x = adamw_one(pv.x, gv.x * gs, mv.x, vv.x, a);
+      pv.y = adamw_one(pv.y, gv.y * gs, mv.y, vv.y, a);
+      pv.z = adamw_one(pv.z, gv.z * gs, mv.z, vv.z, a);
+      pv.w = adamw_one(pv.w, gv.w * gs, mv.w, vv.w, a);
       reinterpret_cast<float4*>(p)[i] = pv;
       reinterpret_cast<float4*>(m)[i] = mv;
       reinterpret_cast<float4*>(v)[i] = vv;
@@ -69,7 +72,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
   }
   for (int64_t i = done + threadIdx.x; i < n; i += 256) {  // ragged tail, or a tensor at an odd address
     float mm = m[i], vv = v[i];
-    const float pn = adamw_one(p[i], g[i], mm, vv, a);
+    const float pn = adamw_one(p[i], g[i] * gs, mm, vv, a);
     p[i] = pn; m[i] = mm; v[i] = vv;
     if (p16 != nullptr) p16[i] = __float2bfloat16(pn);
   }
@@ -79,9 +82,10 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 
 using namespace hawk;
 
-extern "C" int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
-                                float weight_decay, int64_t step, void* stream) {
+extern "C" int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2,
+                                       float eps, float weight_decay, int64_t step, const float* grad_scale, void* stream) {
   HAWK_REQUIRE(tensors, HAWK_ERR_NULL);
+  HAWK_REQUIRE(aligned(grad_scale, 4), HAWK_ERR_ALIGN);
   HAWK_REQUIRE(count >= 1 && step >= 1, HAWK_ERR_SHAPE);
   for (int i = 0; i < count; ++i) {
     const hawk_adamw_tensor& t = tensors[i];
@@ -113,12 +117,17 @@ extern "C" int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, flo
     }
     tab.first[k] = blocks;
     tab.count = k;
-    adamw_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(tab, a);
+    adamw_kernel<<<blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(tab, a, grad_scale);
     const int rc = launch_status();
     if (rc != HAWK_OK) return rc;
     i0 += k;
   }
   return HAWK_OK;
+}
+
+extern "C" int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
+                                float weight_decay, int64_t step, void* stream) {
+  return hawk_adamw_multi_scaled(tensors, count, lr, beta1, beta2, eps, weight_decay, step, nullptr, stream);
 }
 
 extern "C" int hawk_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, float lr,

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import inspect
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -1720,3 +1721,73 @@ def add_rms_norm(res, delta, weight, eps: float = 1e-6, out_dtype=None):
         delta = delta.to(out_dtype)
     new_res, y, _ = add_rms_norm_fwd(res, delta, w32, eps, out_dtype)
     return new_res, y
+
+
+# ---------------------------------------------------------------------------------------------
+# the norm of a model's gradients
+# ---------------------------------------------------------------------------------------------
+def _norm_table(tensors):
+    """(hawk_norm_tensor's of the tensors that hold anything, their device, what has to stay alive until the call is made)"""
+    flat, keep, device = [], [], None
+    for t in tensors:
+        if not t.is_cuda:
+            raise RuntimeError("hawk_b200: tensors must be on a CUDA device (there is no CPU path)")
+        if device is None:
+            device = t.device
+        elif t.device != device:
+            raise RuntimeError(f"hawk_b200: tensors on {device} and {t.device} in one call")
+        if t.layout != torch.strided:
+            raise TypeError(f"hawk_b200: a {t.layout} tensor in a norm")
+        n = t.numel()
+        if n == 0:
+            continue
+        if not t.is_contiguous():
+            t = t.contiguous()
+            keep.append(t)
+        flat += (t.data_ptr(), n, _dt(t))
+    return flat, device, keep
+
+
+def _grad_norm(table, device, max_norm: float) -> torch.Tensor:
+    """fp32 [norm, min(1, max_norm / (norm + 1e-6))] of the tensors in a table of _norm_table."""
+    if not max_norm >= 0:
+        raise ValueError(f"hawk_b200: max_norm {max_norm} (a norm is not negative)")
+    if not table:
+        return torch.tensor([0.0, min(1.0, max_norm / 1e-6)], device=device)
+    lib = _lib.load()
+    count = len(table) // 3
+    out = torch.empty(2, dtype=torch.float32, device=device)
+    ws = torch.empty(lib.hawk_grad_norm_workspace_bytes(count), dtype=torch.uint8, device=device)
+    with _on(out, "grad_norm", (count + 1023) // 1024 + 1):
+        _lib.check(lib.hawk_grad_norm(struct.pack(f"{len(table)}q", *table), count, max_norm, out.data_ptr(), ws.data_ptr(),
+                                      ws.numel(), _stream(out)), "hawk_grad_norm")
+    return out
+
+
+def grad_norm(tensors) -> torch.Tensor:
+    """The 2-norm over all elements of `tensors` (fp32 or bf16, any shapes, one device) as an fp32 scalar on their device, in
+    two launches and without a synchronisation.  Not differentiable.  Deterministic, and right for every norm that fp32 can hold
+    (the squares may leave its range)."""
+    table, device, keep = _norm_table([tensors] if isinstance(tensors, torch.Tensor) else tensors)
+    return _grad_norm(table, device, 0.0)[0]
+
+
+def scale_in_place(tensors, scale: torch.Tensor) -> None:
+    """t *= scale for every t of `tensors` (fp32 or bf16, contiguous, not overlapping), with `scale` an fp32 scalar on their
+    device; nothing is read or written where it is 1."""
+    table, device, keep = _norm_table(tensors)
+    if keep:
+        raise ValueError("hawk_b200: scale_in_place takes contiguous tensors")
+    if not table:
+        return
+    spans = sorted((p, p + n * (2 if d == _lib.HAWK_BF16 else 4)) for p, n, d in zip(table[::3], table[1::3], table[2::3]))
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("hawk_b200: tensors that share memory cannot be scaled in place by one call")
+    if scale.device != device or scale.dtype != torch.float32 or scale.numel() != 1:
+        raise ValueError(f"hawk_b200: scale has to be an fp32 scalar on {device}")
+    lib = _lib.load()
+    count = len(table) // 3
+    with _on(scale, "scale_multi", (count + 1023) // 1024):
+        _lib.check(lib.hawk_scale_multi(struct.pack(f"{len(table)}q", *table), count, scale.data_ptr(), _stream(scale)),
+                   "hawk_scale_multi")
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])  # written behind autograd's back

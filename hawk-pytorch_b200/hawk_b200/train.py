@@ -32,14 +32,46 @@ def init_distributed(backend: Optional[str] = None) -> tuple:
     return rank, local_rank, world
 
 
+def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
+    """Scales the gradients of `parameters` (fp32 or bf16, on one CUDA device) in place so that their global 2-norm is at most
+    `max_norm`, by torch.nn.utils.clip_grad_norm_'s rule: times min(1, max_norm / (norm + 1e-6)).  Returns the norm before, as a
+    scalar on the device; nothing synchronises.  `FusedAdamW(max_grad_norm=)` does the same without a pass of its own."""
+    from . import ops
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads, seen = [], set()
+    for p in parameters:
+        if p.grad is not None and id(p) not in seen:
+            seen.add(id(p))
+            grads.append(p.grad)
+    if not grads:
+        return torch.zeros(())
+    with torch.no_grad():
+        table, device, keep = ops._norm_table(grads)
+        both = ops._grad_norm(table, device, float(max_norm))
+        strided = [g for g in grads if not g.is_contiguous()]
+        if strided:  # neither copied nor listed twice: torch's own product, which knows strides
+            torch._foreach_mul_(strided, both[1])
+        ops.scale_in_place([g for g in grads if g.is_contiguous()], both[1])
+    return both[0]
+
+
 class FusedAdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's update (decoupled weight decay, bias correction) of fp32 parameters, up to 64 tensors
     to a kernel that also writes the bf16 copy of the updated weight for the model's `Linear`
     layers (`shadow_modules`: modules with `.weight`, `.weight_bf16`, `.weight_bf16_version`), so the next
-    forward casts nothing.  State keys follow torch.optim.AdamW (`step`, `exp_avg`, `exp_avg_sq`)."""
+    forward casts nothing.  State keys follow torch.optim.AdamW (`step`, `exp_avg`, `exp_avg_sq`).
 
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, shadow_modules=()):
+    `max_grad_norm`: every step takes the gradients of all groups times min(1, max_grad_norm / (norm + 1e-6)), where norm is
+    their global 2-norm before (`grad_norm` after the step: a scalar on the device).  `p.grad` itself is left as it is: the factor
+    is applied as the update reads it."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, shadow_modules=(),
+                 max_grad_norm: Optional[float] = None):
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError(f"max_grad_norm {max_grad_norm} (a norm is not negative)")
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
         self._shadow = {id(m.weight): m for m in shadow_modules}
 
     @torch.no_grad()
@@ -51,6 +83,13 @@ class FusedAdamW(torch.optim.Optimizer):
                 loss = closure()
         lib = _lib.load()
         touched, keep, launches = [], [], 0
+        clip = None
+        if self.max_grad_norm is not None:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if grads:
+                table, device, kept = ops._norm_table(grads)
+                both = ops._grad_norm(table, device, float(self.max_grad_norm))
+                self.grad_norm, clip = both[0], both.data_ptr() + 4
         for group in self.param_groups:
             b1, b2 = group["betas"]
             lr, eps, wd = group["lr"], group["eps"], group["weight_decay"]
@@ -77,9 +116,9 @@ class FusedAdamW(torch.optim.Optimizer):
                     touched.append(p)
                 for (dev, step), (flat, states) in batches.items():
                     with torch.cuda.device(dev):
-                        rc = lib.hawk_adamw_multi(struct.pack(f"{len(flat)}Q", *flat), len(flat) // 6, lr, b1, b2, eps, wd, step,
-                                                  torch.cuda.current_stream().cuda_stream)
-                    _lib.check(rc, "hawk_adamw_multi")
+                        rc = lib.hawk_adamw_multi_scaled(struct.pack(f"{len(flat)}Q", *flat), len(flat) // 6, lr, b1, b2, eps, wd,
+                                                         step, clip, torch.cuda.current_stream().cuda_stream)
+                    _lib.check(rc, "hawk_adamw_multi_scaled")
                     launches += (len(flat) // 6 + 63) // 64
                     states.clear()
             except BaseException:
@@ -184,17 +223,22 @@ class Trainer:
     cross-entropy with labels = inputs), backward, gradient all-reduce and the optimiser update.
     `grad_comm_dtype`: torch.float32 (default: the gradients are all-reduced as they are) or torch.bfloat16
     (each bucket is rounded to bf16 for the all-reduce and restored: half the NVLink bytes).
-    `timeline`: a CommTimeline that the step fills (multi-GPU only).  `check_status_every`: see below."""
+    `timeline`: a CommTimeline that the step fills (multi-GPU only).  `check_status_every`: see below.
+    `max_grad_norm`: clip the gradients (after their all-reduce) to this global 2-norm; `grad_norm` then holds the norm of the
+    last step, a scalar on the device."""
 
     def __init__(self, config: HawkConfig, device, seed: int = 0, lr: float = 3e-4, world_size: int = 1,
                  autocast: bool = True, bucket_cap_mb: int = 256, grad_comm_dtype: torch.dtype = torch.float32,
-                 timeline: Optional[CommTimeline] = None, check_status_every: int = 100):
+                 timeline: Optional[CommTimeline] = None, check_status_every: int = 100,
+                 max_grad_norm: Optional[float] = None):
         torch.manual_seed(seed)  # same seed on every rank: identical replicas
         self.device = torch.device(device)
         self.model = HawkModel(config).to(self.device)
         self.autocast = autocast and self.device.type == "cuda"
         self.ddp = None
         self.steps_done = 0
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
         # every this many steps the device status word of the tensor-core kernels is read back (one host sync):
         # a kernel that gave up a bounded wait then raises here instead of training on (its loss is NaN anyway)
         self.check_status_every = check_status_every
@@ -209,10 +253,21 @@ class Trainer:
         if self.device.type == "cuda":
             from .model import Linear
             shadows = [m for m in self.model.modules() if isinstance(m, Linear) and m.bias is None] if self.autocast else []
-            self.opt = FusedAdamW(self.model.parameters(), lr=lr, weight_decay=0.1, shadow_modules=shadows)
+            self.opt = FusedAdamW(self.model.parameters(), lr=lr, weight_decay=0.1, shadow_modules=shadows,
+                                  max_grad_norm=max_grad_norm)
         else:
             self.opt = torch.optim.AdamW(self.model.parameters(), lr=lr, weight_decay=0.1,
                                          fused=self.device.type == "cuda")
+
+    def _update(self) -> None:
+        if isinstance(self.opt, FusedAdamW):
+            self.opt.step()
+            self.grad_norm = self.opt.grad_norm
+        else:
+            if self.max_grad_norm is not None:
+                self.grad_norm = torch.nn.utils.clip_grad_norm_(self.model.parameters(), self.max_grad_norm)
+            self.opt.step()
+        self.opt.zero_grad(set_to_none=True)
 
     def step(self, ids: torch.Tensor, after_backward=None, sync_gradients: bool = True) -> torch.Tensor:
         """One training step; `after_backward(loss)`, when given, runs between the backward pass (gradients
@@ -225,8 +280,7 @@ class Trainer:
                 with torch.autocast(self.device.type, dtype=torch.bfloat16, enabled=self.autocast):
                     loss = net(ids, ids)
                 loss.backward()
-            self.opt.step()
-            self.opt.zero_grad(set_to_none=True)
+            self._update()
             self.steps_done += 1
             return loss.detach()
         with torch.autocast(self.device.type, dtype=torch.bfloat16, enabled=self.autocast):
@@ -236,8 +290,7 @@ class Trainer:
         loss.backward()
         if after_backward is not None:
             after_backward(loss.detach())
-        self.opt.step()
-        self.opt.zero_grad(set_to_none=True)
+        self._update()
         self.steps_done += 1
         if self.check_status_every > 0 and self.steps_done % self.check_status_every == 0 and self.device.type == "cuda":
             from . import ops

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define HAWK_B200_ABI_VERSION 6
+#define HAWK_B200_ABI_VERSION 7
 
 typedef enum hawk_dtype { HAWK_F32 = 0, HAWK_BF16 = 1 } hawk_dtype;
 
@@ -373,6 +373,24 @@ typedef struct hawk_adamw_tensor {
 } hawk_adamw_tensor;
 int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
                      float weight_decay, int64_t step, void* stream);
+/* The same with the gradients taken times *grad_scale (a device scalar, e.g. the second result of hawk_grad_norm; NULL = 1). */
+int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
+                            float weight_decay, int64_t step, const float* grad_scale, void* stream);
+
+/* The 2-norm over all elements of `count` tensors (a host array, n >= 1 contiguous elements each, fp32 or bf16), and the
+ * factor that clips them to max_norm >= 0: out[0] = norm, out[1] = min(1, max_norm / (norm + 1e-6)) (NaN where the norm is).
+ * Deterministic; squares that leave fp32's range are formed in double.  Workspace: 8-byte aligned,
+ * hawk_grad_norm_workspace_bytes(count).  hawk_scale_multi multiplies the tensors by *scale in place and touches nothing
+ * where *scale is 1; its tensors must not overlap.  No counterpart in the reference (torch.nn.utils.clip_grad_norm_'s rule). */
+typedef struct hawk_norm_tensor {
+  const void* x;
+  int64_t n;
+  int64_t dtype;
+} hawk_norm_tensor;
+size_t hawk_grad_norm_workspace_bytes(int count);
+int hawk_grad_norm(const hawk_norm_tensor* tensors, int count, float max_norm, float* out, void* workspace,
+                   size_t workspace_bytes, void* stream);
+int hawk_scale_multi(const hawk_norm_tensor* tensors, int count, const float* scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,60 @@
+"""Argument checks of the embedding, log-probability and gradient-norm entry points; no GPU needed."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+import hawk_b200._lib as L
+
+
+def _table(*rows):
+    return struct.pack(f"{3 * len(rows)}q", *(v for r in rows for v in r))
+
+
+def test_grad_norm_argument_validation():
+    lib = L.load()
+    p = ctypes.c_void_p(4096)  # never dereferenced: validation fails first
+    good = _table((4096, 8, 0))
+    ws = lib.hawk_grad_norm_workspace_bytes(1)
+    assert lib.hawk_grad_norm(None, 1, 1.0, p, p, ws, None) == -1
+    assert lib.hawk_grad_norm(good, 1, 1.0, None, p, ws, None) == -1
+    assert lib.hawk_grad_norm(good, 0, 1.0, p, p, ws, None) == -2
+    assert lib.hawk_grad_norm(good, 1, -1.0, p, p, ws, None) == -2
+    assert lib.hawk_grad_norm(good, 1, float("nan"), p, p, ws, None) == -2
+    assert lib.hawk_grad_norm(good, 1, 1.0, p, None, ws, None) == -5
+    assert lib.hawk_grad_norm(good, 1, 1.0, p, p, ws - 1, None) == -5
+    assert lib.hawk_grad_norm(good, 1, 1.0, p, ctypes.c_void_p(4100), ws, None) == -4
+    for row, code in [((0, 8, 0), -1), ((4096, 0, 0), -2), ((4096, 8, 2), -3), ((4098, 8, 0), -4), ((4097, 8, 1), -4),
+                      ((4096, 1 << 41, 0), -2)]:
+        assert lib.hawk_grad_norm(_table(row), 1, 1.0, p, p, ws, None) == code
+        assert lib.hawk_scale_multi(_table(row), 1, p, None) == code
+    assert lib.hawk_grad_norm(_table(*[(4096, 1 << 40, 0)] * 64), 64, 1.0, p, p, ws, None) == -2  # beyond 32 bits of chunks
+    assert lib.hawk_scale_multi(good, 1, None, None) == -1
+    assert lib.hawk_scale_multi(good, 1, ctypes.c_void_p(4098), None) == -4
+    assert lib.hawk_grad_norm_workspace_bytes(1025) == 2 * lib.hawk_grad_norm_workspace_bytes(1024)
+    adam = (1e-3, 0.9, 0.999, 1e-8, 0.1)
+    one = struct.pack("6Q", 4096, 4096, 4096, 4096, 0, 8)
+    assert lib.hawk_adamw_multi_scaled(one, 1, *adam, 1, ctypes.c_void_p(4098), None) == -4
+
+
+def test_norm_refuses_cpu_tensors():
+    from hawk_b200 import grad_norm
+    with pytest.raises(RuntimeError, match="CUDA"):
+        grad_norm([torch.ones(3)])
+
+
+def test_cpu_trainer_clips():
+    """The plumbing of max_grad_norm where the trainer runs torch's own optimiser (no kernels on the CPU)."""
+    from hawk_b200.train import Trainer
+    tr = Trainer.__new__(Trainer)
+    tr.model = torch.nn.Linear(4, 3)
+    tr.opt = torch.optim.SGD(tr.model.parameters(), lr=1.0)
+    tr.max_grad_norm, tr.grad_norm = 0.5, None
+    before = [p.detach().clone() for p in tr.model.parameters()]
+    for p in tr.model.parameters():
+        p.grad = torch.ones_like(p)
+    tr._update()
+    assert abs(float(tr.grad_norm) - 15 ** 0.5) < 1e-6
+    moved = torch.cat([(b - p.detach()).view(-1) for b, p in zip(before, tr.model.parameters())])
+    assert abs(float(moved.norm()) - 0.5) < 1e-5 and all(p.grad is None for p in tr.model.parameters())

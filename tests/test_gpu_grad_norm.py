@@ -1,0 +1,198 @@
+"""The global gradient norm, clipping and the clipped optimiser step against the same in 64 bits.
+
+Tolerances: the norm is one fp32 rounding of a sum whose terms are right to 8 roundings of 2^-24 each, summed in double:
+under 1e-6 relative.  A clipped gradient is the rounding of g * coef, coef itself rounded: 2 * eps / 2 of the type plus
+2^-24; an AdamW step on fp32 tensors is held to the bound of its own test."""
+import math
+
+import pytest
+import torch
+
+from conftest import rel_l2
+
+pytestmark = pytest.mark.gpu
+
+
+def _list(seed, dtypes=(torch.float32, torch.bfloat16), count=40):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    out = []
+    for i in range(count):
+        n = [1, 7, 8, 255, 8191, 8192, 8193, 16385, 100003, 513 * 129][i % 10]
+        out.append((torch.randn(n, generator=g, device="cuda") * 10.0 ** (i % 5 - 3)).to(dtypes[i % len(dtypes)]))
+    return out
+
+
+def _norm64(ts):
+    return math.sqrt(sum(float(t.double().square().sum()) for t in ts))
+
+
+@pytest.mark.parametrize("count", [1, 2, 40, 128, 129, 1023, 1024, 1025, 2100])
+def test_norm_of_lists(count):
+    from hawk_b200 import grad_norm
+    ts = _list(count, count=count)
+    got = grad_norm(ts)
+    assert got.shape == () and got.dtype == torch.float32
+    assert abs(float(got) - _norm64(ts)) <= 1e-6 * _norm64(ts)
+    assert torch.equal(got, grad_norm(ts))
+
+
+def test_norm_of_views_and_empty_tensors():
+    from hawk_b200 import grad_norm
+    base = torch.randn(3000, 7, device="cuda")
+    ts = [base[1:].view(-1)[1:], base.t(), base[::3], torch.empty(0, device="cuda"), base.bfloat16().view(-1)[3:]]
+    assert abs(float(grad_norm(ts)) - _norm64(ts)) <= 1e-6 * _norm64(ts)
+    assert float(grad_norm([torch.empty(0, 4, device="cuda")])) == 0.0
+    assert float(grad_norm([torch.zeros(9, device="cuda")])) == 0.0
+    assert abs(float(grad_norm(base)) - _norm64([base])) <= 1e-6 * _norm64([base])  # a tensor by itself
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-22, 1e18, 1e30, 1e37])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_norm_beyond_the_range_of_squares(scale, dtype):
+    from hawk_b200 import grad_norm
+    t = (torch.rand(5001, device="cuda") * scale).to(dtype)
+    got, norm = float(grad_norm([t])), _norm64([t])
+    # 5001 values of 1e37 have a norm of sqrt(5001 / 3) 1e37 = 4.1e38, above fp32's largest 3.403e38: its rounding is infinity
+    want = float(torch.tensor(norm, dtype=torch.float64).float())
+    assert got == want if math.isinf(want) else abs(got - norm) <= 1e-6 * norm
+
+
+def test_norm_of_non_finite_values():
+    from hawk_b200 import grad_norm
+    a, b = torch.randn(100, device="cuda"), torch.randn(33000, device="cuda").bfloat16()
+    b[32999] = math.inf
+    assert float(grad_norm([a, b])) == math.inf
+    a[3] = math.nan
+    assert math.isnan(float(grad_norm([a, b])))
+
+
+@pytest.mark.parametrize("share", [0.0, 0.25, 2.0, math.inf])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_clip_matches_the_rule(share, dtype):
+    from hawk_b200.train import clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(t.shape, dtype=dtype, device="cuda")) for t in _list(3)]
+    for p, t in zip(ps, _list(3)):
+        p.grad = t.to(dtype)
+    ps.append(torch.nn.Parameter(torch.zeros(70, 30, dtype=dtype, device="cuda")))
+    ps[-1].grad = torch.randn(30, 70, device="cuda").to(dtype).t()   # a gradient that is not contiguous
+    ps.append(torch.nn.Parameter(torch.zeros(3, device="cuda")))     # and a parameter without one
+    had = [p.grad.clone() for p in ps[:-1]]
+    norm = _norm64(had)
+    version = ps[0].grad._version
+    got = clip_grad_norm_(ps + ps[:1], share * norm)                 # a parameter named twice counts once
+    assert abs(float(got) - norm) <= 1e-6 * norm and ps[0].grad._version > version
+    coef = min(1.0, share * norm / (norm + 1e-6))
+    for p, h in zip(ps, had):
+        if coef == 1.0:
+            assert torch.equal(p.grad, h)
+        else:
+            bound = torch.finfo(dtype).eps / 2 + 4 * 2.0 ** -24
+            assert bool(((p.grad.double() - h.double() * coef).abs() <= bound * (h.double() * coef).abs() + 1e-38).all())
+
+
+def test_clip_makes_every_gradient_nan_when_one_is():
+    from hawk_b200.train import clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(5, device="cuda")) for _ in range(2)]
+    ps[0].grad, ps[1].grad = torch.ones(5, device="cuda"), torch.full((5,), math.nan, device="cuda")
+    assert math.isnan(float(clip_grad_norm_(ps, 1.0))) and bool(ps[0].grad.isnan().all())  # as torch's
+
+
+def test_refusals():
+    from hawk_b200 import grad_norm, ops
+    from hawk_b200.train import FusedAdamW, clip_grad_norm_
+    a = torch.ones(8, device="cuda")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        grad_norm([a, torch.ones(3)])
+    with pytest.raises(TypeError, match="float16"):
+        grad_norm([a.half()])
+    with pytest.raises(ValueError, match="share memory"):
+        ops.scale_in_place([a, a[2:]], torch.ones((), device="cuda"))
+    with pytest.raises(ValueError, match="scalar"):
+        ops.scale_in_place([a], torch.ones(2, device="cuda"))
+    p = torch.nn.Parameter(a)
+    p.grad = a.clone()
+    for bad in (-1.0, math.nan):
+        with pytest.raises(ValueError, match="max_norm"):
+            clip_grad_norm_([p], bad)
+        with pytest.raises(ValueError, match="max_grad_norm"):
+            FusedAdamW([p], max_grad_norm=bad)
+
+
+@pytest.mark.parametrize("max_norm", [0.5, 1e9])
+def test_clipped_adamw_matches_torch(max_norm):
+    from hawk_b200.train import FusedAdamW
+    shapes = [(33, 65), (8193,), (4, 128), (1,)]
+    torch.manual_seed(0)
+    ours = [torch.nn.Parameter(torch.randn(s, device="cuda")) for s in shapes]
+    ref = [torch.nn.Parameter(p.detach().double().clone()) for p in ours]
+    groups = lambda ps: [dict(params=ps[:2]), dict(params=ps[2:], lr=1e-2)]  # noqa: E731
+    opt = FusedAdamW(groups(ours), lr=1e-3, weight_decay=0.1, max_grad_norm=max_norm)
+    topt = torch.optim.AdamW(groups(ref), lr=1e-3, weight_decay=0.1)
+    for _ in range(4):
+        for p, q in zip(ours, ref):
+            g = torch.randn(p.shape, device="cuda")
+            p.grad, q.grad = g, g.double()
+        norm = torch.nn.utils.clip_grad_norm_(ref, max_norm)
+        kept = [p.grad.clone() for p in ours]
+        opt.step()
+        topt.step()
+        assert abs(float(opt.grad_norm) - float(norm)) <= 1e-6 * float(norm)
+        assert all(torch.equal(p.grad, k) for p, k in zip(ours, kept))  # the gradients stay as they were
+    for p, q in zip(ours, ref):
+        assert rel_l2(p.detach(), q.detach()) <= 2e-6
+
+
+def test_unclipped_adamw_is_unchanged_by_a_large_bound():
+    from hawk_b200.train import FusedAdamW
+    torch.manual_seed(1)
+    a = [torch.nn.Parameter(torch.randn(5000, device="cuda")) for _ in range(3)]
+    b = [torch.nn.Parameter(p.detach().clone()) for p in a]
+    oa, ob = FusedAdamW(a), FusedAdamW(b, max_grad_norm=1e30)
+    for p, q in zip(a, b):
+        p.grad = q.grad = torch.randn(5000, device="cuda")
+    oa.step()
+    ob.step()
+    assert all(torch.equal(p, q) for p, q in zip(a, b)) and oa.grad_norm is None
+
+
+def test_captured_norm_follows_its_inputs():
+    from hawk_b200 import grad_norm
+    ts = _list(9, count=130)
+    grad_norm(ts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = grad_norm(ts)
+    for k in (1.0, 3.0):
+        for t in ts:
+            t.mul_(k)
+        graph.replay()
+        assert abs(float(got) - _norm64(ts)) <= 1e-6 * _norm64(ts)
+
+
+def test_norm_on_another_stream():
+    from hawk_b200 import grad_norm
+    ts = _list(4)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for t in ts:
+            t.mul_(2.0)
+        got = grad_norm(ts)
+    torch.cuda.current_stream().wait_stream(side)
+    assert abs(float(got) - _norm64(ts)) <= 1e-6 * _norm64(ts)
+
+
+def test_trainer_clips():
+    import hawk_b200.model as M
+    from hawk_b200.train import Trainer
+    cfg = M.HawkConfig(96, 64, 128, 2, 64, 4, 4)
+    ids = torch.randint(1, 96, (2, 33), device="cuda")
+    tr = Trainer(cfg, "cuda", seed=3, max_grad_norm=0.25)
+    grads = []
+    tr.step(ids, after_backward=lambda _: grads.extend(p.grad.clone() for p in tr.model.parameters()))
+    assert abs(float(tr.grad_norm) - _norm64(grads)) <= 1e-6 * _norm64(grads)
+    first = next(p for p in tr.model.parameters() if p.dim() == 2)
+    st = tr.opt.state[first]
+    coef = min(1.0, 0.25 / (_norm64(grads) + 1e-6))
+    assert rel_l2(st["exp_avg"], 0.1 * coef * grads[0].double()) <= 1e-6

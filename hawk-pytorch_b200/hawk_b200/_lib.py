@@ -63,6 +63,9 @@ SIGNATURES = {
     "hawk_grad_norm_workspace_bytes": (c_size_t, [c_int]),
     "hawk_grad_norm": (c_int, [c_char_p, c_int, c_float, _P, _P, c_size_t, _P]),
     "hawk_scale_multi": (c_int, [c_char_p, c_int, _P, _P]),
+    "hawk_embedding_fwd": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_float, c_int, _P]),
+    "hawk_embedding_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "hawk_embedding_bwd": (c_int, [_P, _P, _P, _P, c_size_t, c_int64, c_int64, c_int64, c_int64, c_float, c_int, _P]),
     "hawk_scale": (c_int, [_P, _P, _P, c_int64, c_int, _P]),
     "hawk_cast_f32_bf16": (c_int, [_P, _P, c_int64, _P]),
     "hawk_gelu_mul_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int, c_int, _P]),

@@ -204,6 +204,25 @@ def drop_bf16_copies(module: nn.Module) -> None:
             m.drop_bf16_copy()
 
 
+class Embedding(nn.Embedding):
+    """nn.Embedding (same parameter name and state-dict key, hawk/hawk.py:262) on `ops.embedding` for CUDA tables in fp32 or bf16:
+    `scale` multiplies the rows in the same pass (1, the reference's model, leaves them as they are; models of this family also
+    use sqrt(width)), and the gradient is summed by token in a fixed order.  `max_norm`, `scale_grad_by_freq` and `sparse` are
+    nn.Embedding's own code."""
+
+    def __init__(self, *args, scale: float = 1.0, **kwargs):
+        super().__init__(*args, **kwargs)
+        self.scale = scale
+
+    def forward(self, ids):
+        w = self.weight
+        if (not w.is_cuda or w.dtype not in (torch.float32, torch.bfloat16) or self.max_norm is not None or self.scale_grad_by_freq
+                or self.sparse):
+            out = super().forward(ids)
+            return out if self.scale == 1.0 else out * self.scale
+        return ops.embedding(ids, w, self.scale, self.padding_idx)
+
+
 class MLP(nn.Module):
     """Gated GELU feed-forward (hawk/hawk.py:61-86); `resid_proj` starts at zero."""
 
@@ -426,7 +445,7 @@ class HawkModel(nn.Module):
         super().__init__()
         self.config = config
         self.use_cache = use_cache
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size)
+        self.embed_tokens = Embedding(config.vocab_size, config.hidden_size)
         self.layers = nn.ModuleList(RNNLayer(config, use_cache) for _ in range(config.num_hidden_layers))
         self.norm = RMSNorm(config.hidden_size)
         self.lm_head = nn.Linear(config.hidden_size, config.vocab_size, bias=False)

@@ -1724,6 +1724,97 @@ def add_rms_norm(res, delta, weight, eps: float = 1e-6, out_dtype=None):
 
 
 # ---------------------------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------------------------
+@_operator("hawk_b200::embedding_fwd", mutates_args=())
+def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: int = -1) -> torch.Tensor:
+    """scale * weight[ids], in weight's dtype; ids int64 of any shape."""
+    _same_device(weight, ids)
+    lib = _lib.load()
+    ids, weight = ids.contiguous(), weight.contiguous()
+    V, H = weight.shape
+    out = torch.empty((*ids.shape, H), dtype=weight.dtype, device=weight.device)
+    if out.numel():
+        with _on(weight, "embedding_fwd", 1):
+            _lib.check(lib.hawk_embedding_fwd(ids.data_ptr(), weight.data_ptr(), out.data_ptr(), ids.numel(), V, H, scale, _dt(weight),
+                                              _stream(weight)), "hawk_embedding_fwd")
+    return out
+
+
+@embedding_fwd.register_fake
+def _(ids, weight, scale=1.0, padding_idx=-1):
+    return weight.new_empty((*ids.shape, weight.shape[1]))
+
+
+@_operator("hawk_b200::embedding_bwd", mutates_args=())
+def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, V: int, scale: float, padding_idx: int) -> torch.Tensor:
+    """The gradient of embedding_fwd's weight, [V, H] in dout's dtype."""
+    _same_device(dout, ids)
+    lib = _lib.load()
+    ids, dout = ids.contiguous(), dout.contiguous()
+    N, H = ids.numel(), dout.shape[-1]
+    if N == 0 or H == 0:
+        return torch.zeros(V, H, dtype=dout.dtype, device=dout.device)
+    dw = torch.empty(V, H, dtype=dout.dtype, device=dout.device)
+    ws = torch.empty(lib.hawk_embedding_bwd_workspace_bytes(N, V, H), dtype=torch.uint8, device=dout.device)
+    with _on(dout, "embedding_bwd", 3 if N > 64 else 2):
+        _lib.check(lib.hawk_embedding_bwd(ids.data_ptr(), dout.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), N, V, H,
+                                          padding_idx, scale, _dt(dout), _stream(dout)), "hawk_embedding_bwd")
+    return dw
+
+
+@embedding_bwd.register_fake
+def _(ids, dout, V, scale, padding_idx):
+    return dout.new_empty(V, dout.shape[-1])
+
+
+def _embed_setup(ctx, inputs, output):
+    ids, weight, ctx.scale, ctx.padding_idx = inputs
+    ctx.save_for_backward(ids)
+    ctx.V = weight.shape[0]
+
+
+def _embed_backward(ctx, dout):
+    return None, embedding_bwd(ctx.saved_tensors[0], dout, ctx.V, ctx.scale, ctx.padding_idx), None, None
+
+
+embedding_fwd.register_autograd(_embed_backward, setup_context=_embed_setup)
+
+
+def _embed_bwd_setup(ctx, inputs, output):
+    ids, _, V, ctx.scale, ctx.padding_idx = inputs
+    ctx.save_for_backward(ids)
+
+
+def _embed_bwd_backward(ctx, ddw):  # linear in dout: its rows are those of ddw, nothing where padding_idx kept one out
+    ids, = ctx.saved_tensors
+    rows = embedding_fwd(ids, ddw, ctx.scale)
+    return None, rows.masked_fill((ids == ctx.padding_idx)[..., None], 0.0), None, None, None
+
+
+embedding_bwd.register_autograd(_embed_bwd_backward, setup_context=_embed_bwd_setup)
+
+
+def embedding(ids, weight, scale: float = 1.0, padding_idx: Optional[int] = None):
+    """scale * weight[ids] (weight [V,H] fp32 or bf16, ids of any shape and integer type), in weight's dtype.  The gradient of
+    `weight` is dense, summed in fp32 in the order of the positions (the same bits on every run) and rounded once; the row
+    `padding_idx` gets none.  An id outside [0, V) gives a row of NaN and no gradient."""
+    if weight.dim() != 2:
+        raise ValueError(f"hawk_b200: an embedding table has two dimensions, not {weight.dim()}")
+    if ids.dtype != torch.int64:
+        if ids.dtype.is_floating_point or ids.dtype.is_complex or ids.dtype == torch.bool:
+            raise TypeError(f"hawk_b200: token ids are integers, not {ids.dtype}")
+        ids = ids.long()
+    if padding_idx is None:
+        padding_idx = -1
+    else:
+        if not -weight.shape[0] <= padding_idx < weight.shape[0]:
+            raise ValueError(f"hawk_b200: padding_idx {padding_idx} with a table of {weight.shape[0]} rows")
+        padding_idx %= weight.shape[0]
+    return embedding_fwd(ids, weight, float(scale), padding_idx)
+
+
+# ---------------------------------------------------------------------------------------------
 # the norm of a model's gradients
 # ---------------------------------------------------------------------------------------------
 def _norm_table(tensors):

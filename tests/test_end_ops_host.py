@@ -58,3 +58,29 @@ def test_cpu_trainer_clips():
     assert abs(float(tr.grad_norm) - 15 ** 0.5) < 1e-6
     moved = torch.cat([(b - p.detach()).view(-1) for b, p in zip(before, tr.model.parameters())])
     assert abs(float(moved.norm()) - 0.5) < 1e-5 and all(p.grad is None for p in tr.model.parameters())
+
+
+def test_embedding_argument_validation():
+    lib = L.load()
+    p = ctypes.c_void_p(4096)
+    assert lib.hawk_embedding_fwd(None, p, p, 4, 10, 8, 1.0, 0, None) == -1
+    assert lib.hawk_embedding_fwd(p, p, p, 0, 10, 8, 1.0, 0, None) == -2
+    assert lib.hawk_embedding_fwd(p, p, p, 4, 10, 0, 1.0, 0, None) == -2
+    assert lib.hawk_embedding_fwd(p, p, p, 4, 1 << 31, 8, 1.0, 0, None) == -2
+    assert lib.hawk_embedding_fwd(p, p, p, 1 << 31, 10, 8, 1.0, 0, None) == -2
+    assert lib.hawk_embedding_fwd(p, p, p, 4, 10, 8, 1.0, 5, None) == -3
+    assert lib.hawk_embedding_fwd(p, ctypes.c_void_p(4098), p, 4, 10, 8, 1.0, 0, None) == -4
+    ws = lib.hawk_embedding_bwd_workspace_bytes(100, 10, 8)
+    assert ws >= 100 * 4 + 11 * 4 + 3 * 8 * 4
+    assert lib.hawk_embedding_bwd(p, p, p, None, ws, 100, 10, 8, -1, 1.0, 0, None) == -5
+    assert lib.hawk_embedding_bwd(p, p, p, p, ws - 1, 100, 10, 8, -1, 1.0, 0, None) == -5
+    assert lib.hawk_embedding_bwd(p, p, p, ctypes.c_void_p(4100), ws, 100, 10, 8, -1, 1.0, 0, None) == -4
+    assert lib.hawk_embedding_bwd(p, None, p, p, ws, 100, 10, 8, -1, 1.0, 0, None) == -1
+
+
+def test_embedding_refuses_cpu_tensors():
+    from hawk_b200 import embedding
+    with pytest.raises(RuntimeError, match="CUDA"):
+        embedding(torch.zeros(3, dtype=torch.int64), torch.ones(4, 8))
+    with pytest.raises(TypeError, match="integers"):
+        embedding(torch.zeros(3), torch.ones(4, 8))

@@ -1,0 +1,176 @@
+"""The embedding and its gradient by token against plain ones in 64 bits.
+
+Tolerances.  Forward: one product rounded to fp32 and, in bf16, once more: eps / 2 of the type plus 2^-24, relative.
+Gradient: a sum of c rows in fp32 in order, at most (c - 1) 2^-24 sum |row| off, times the scale (2^-24), rounded to the type."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def _zipf(n, V, g):
+    return (float(V) ** torch.rand(n, generator=g, device="cuda", dtype=torch.float64)).long().sub_(1).clamp_(0, V - 1)
+
+
+def _check(ids, V, H, dtype, scale=1.0, padding=None, seed=0):
+    from hawk_b200 import embedding
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    w = torch.randn(V, H, generator=g, device="cuda").to(dtype).requires_grad_()
+    out = embedding(ids, w, scale, padding)
+    assert out.shape == (*ids.shape, H) and out.dtype == dtype
+    half = torch.finfo(dtype).eps / 2
+    want = w.detach().double()[ids] * scale
+    assert bool(((out.double() - want).abs() <= (half + 2.0 ** -24) * want.abs()).all())
+    go = torch.randn(out.shape, generator=g, device="cuda").to(dtype)
+    dw, = torch.autograd.grad(out, w, go, retain_graph=True)
+    again, = torch.autograd.grad(out, w, go)
+    assert dw.dtype == dtype and torch.equal(dw, again)
+    flat, rows = ids.reshape(-1), go.reshape(-1, H).double()
+    if padding is not None:
+        rows = torch.where((flat == padding % V)[:, None], 0, rows)
+    sums = torch.zeros(V, H, dtype=torch.float64, device="cuda").index_add_(0, flat, rows)
+    mags = torch.zeros(V, H, dtype=torch.float64, device="cuda").index_add_(0, flat, rows.abs())
+    counts = torch.zeros(V, dtype=torch.float64, device="cuda").index_add_(0, flat, torch.ones_like(flat, dtype=torch.float64))
+    bound = (half + 2.0 ** -23) * (sums * scale).abs() + counts[:, None] * 2.0 ** -24 * mags * abs(scale) * (1 + 2 * half)
+    assert bool(((dw.double() - sums * scale).abs() <= bound).all())
+    assert bool((dw[counts == 0] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,H", [(1, 1, 1), (1, 300, 64), (31, 7, 5), (64, 1, 24), (65, 1, 24), (129, 3, 2), (1551, 32000, 512),
+                                   (4097, 1000, 2048), (8192, 50, 36), (8193, 129, 250), (20000, 5000, 1001), (3000, 70001, 8)])
+def test_embedding_matches(n, V, H, dtype):
+    g = torch.Generator(device="cuda").manual_seed(n + V + H)
+    _check(_zipf(n, V, g), V, H, dtype, scale=1.0 if n % 2 else 22.6)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n", [63, 64, 65, 96, 97, 8191, 8192, 8193, 40000])
+def test_one_token_everywhere(n, dtype):
+    """All positions of one block's slice, past its queue; runs that end inside, at and after a window."""
+    _check(torch.full((n,), 11, device="cuda"), 40, 72, dtype)
+
+
+@pytest.mark.parametrize("lead", [0, 1, 31, 32, 33, 63])
+def test_runs_across_windows(lead):
+    ids = torch.cat([torch.zeros(lead, dtype=torch.int64), torch.full((200,), 5), torch.full((64,), 6), torch.full((65,), 8),
+                     torch.arange(9, 30)]).cuda()
+    _check(ids, 30, 40, F32)
+    _check(ids[torch.randperm(ids.numel(), device="cuda")].view(1, -1), 30, 40, BF16)
+
+
+def test_every_vocabulary_slice_width():
+    for V in (31, 32, 33, 147 * 32, 148 * 32 + 1, 148 * 100 + 3, 148 * 4096 + 17):
+        g = torch.Generator(device="cuda").manual_seed(V)
+        _check(torch.randint(0, V, (777,), generator=g, device="cuda"), V, 4, F32)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_padding_and_strangers(dtype):
+    from hawk_b200 import embedding
+    g = torch.Generator(device="cuda").manual_seed(5)
+    ids = _zipf(999, 200, g).view(3, 333)
+    _check(ids, 200, 33, dtype, scale=0.5, padding=0)
+    _check(ids, 200, 32, dtype, padding=-200)
+    w = torch.randn(10, 16, device="cuda").to(dtype).requires_grad_()
+    odd = torch.tensor([3, -1, 10, 2 ** 40, 9, -2 ** 62], device="cuda")
+    out = embedding(odd, w)
+    assert out.isnan().all(1).tolist() == [False, True, True, True, False, True]
+    dw, = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert dw.sum(1).tolist() == [16.0 if i in (3, 9) else 0.0 for i in range(10)]
+
+
+def test_strides_types_and_empty_calls():
+    from hawk_b200 import embedding
+    base = torch.randn(51, 40, device="cuda")
+    ids = torch.randint(0, 50, (6, 10), device="cuda")
+    for w in (base[:50], base[1:], base[:50, :39], base.view(-1)[1:2001].view(50, 40), base.t()[:, :40]):  # odd addresses and strides
+        w = w.detach().requires_grad_()
+        k = ids % w.shape[0]
+        out = embedding(k.t(), w, 2.0)
+        assert torch.equal(out, w.detach()[k.t()] * 2.0)
+        dw, = torch.autograd.grad(out, w, torch.ones(1, device="cuda").expand(out.shape))  # a broadcast gradient
+        assert torch.equal(dw[:, 0], 2.0 * torch.bincount(k.view(-1), minlength=w.shape[0]).float())
+    w = base.detach().requires_grad_()
+    assert torch.equal(embedding(ids.int(), w), embedding(ids, w)) and embedding(ids.to(torch.uint8), w).shape == (6, 10, 40)
+    out = embedding(ids[:0], w)
+    dw, = torch.autograd.grad(out, w, out)
+    assert out.shape == (0, 10, 40) and dw.shape == w.shape and float(dw.abs().max()) == 0.0
+    assert embedding(ids[0, 0], w).shape == (40,)
+
+
+def test_gradient_of_the_gradient():
+    from hawk_b200 import embedding
+    w = torch.randn(6, 4, device="cuda", requires_grad=True)
+    ids = torch.tensor([1, 3, 1, 5, 0], device="cuda")
+    out = embedding(ids, w, 2.0, padding_idx=0)
+    go = torch.randn_like(out).requires_grad_()
+    dw, = torch.autograd.grad(out, w, go, create_graph=True)
+    u = torch.randn_like(dw)
+    dgo, = torch.autograd.grad(dw, go, u)
+    want = 2.0 * u[ids]
+    want[4] = 0
+    assert torch.equal(dgo, want)
+
+
+def test_refusals():
+    from hawk_b200 import embedding
+    w, ids = torch.randn(9, 4, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError, match="integers"):
+        embedding(ids.float(), w)
+    with pytest.raises(ValueError, match="two dimensions"):
+        embedding(ids, w[0])
+    with pytest.raises(ValueError, match="padding_idx"):
+        embedding(ids, w, padding_idx=9)
+    with pytest.raises(TypeError, match="float16"):
+        embedding(ids, w.half())
+    with pytest.raises(RuntimeError, match="cpu"):
+        embedding(ids.cpu(), w)
+
+
+def test_captured_and_other_streams():
+    from hawk_b200 import embedding
+    g = torch.Generator(device="cuda").manual_seed(2)
+    w = torch.randn(500, 96, device="cuda")
+    ids = _zipf(700, 500, g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first = embedding(ids, w, 3.0)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, w[ids] * 3.0)
+    from hawk_b200 import ops
+    graph = torch.cuda.CUDAGraph()
+    go = torch.randn(700, 96, device="cuda")
+    with torch.cuda.graph(graph):
+        out, dw = embedding(ids, w, 3.0), ops.embedding_bwd(ids, go, 500, 3.0, -1)
+    ids.copy_(_zipf(700, 500, g))
+    graph.replay()
+    assert torch.equal(out, w[ids] * 3.0) and torch.equal(dw, ops.embedding_bwd(ids, go, 500, 3.0, -1))
+
+
+def test_module_and_model():
+    import hawk_b200.model as M
+    from hawk_b200 import ops
+    torch.manual_seed(0)
+    e = M.Embedding(50, 24, padding_idx=3, scale=24 ** 0.5).cuda()
+    plain = torch.nn.Embedding(50, 24, padding_idx=3).cuda()
+    plain.load_state_dict(e.state_dict())
+    ids = torch.randint(0, 50, (5, 9), device="cuda")
+    go = torch.randn(5, 9, 24, device="cuda")
+    e(ids).backward(go)
+    (plain(ids) * 24 ** 0.5).backward(go)
+    assert torch.allclose(e.weight.grad, plain.weight.grad, rtol=1e-5, atol=1e-5) and float(e.weight.grad[3].abs().max()) == 0
+    model = M.HawkModel(M.HawkConfig(96, 64, 128, 1, 64, 4, 4)).cuda()
+    ops.LOG.reset()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        model(ids, ids).backward()
+    counts = dict(ops.LOG.counts)
+    ops.LOG.enabled = False
+    assert counts["embedding_fwd"] == 1 and counts["embedding_bwd"] == 2
+    cpu = M.Embedding(50, 24, scale=2.0)
+    assert torch.equal(cpu(ids.cpu()), 2.0 * cpu.weight[ids.cpu()])
+    sparse = M.Embedding(50, 24, sparse=True).cuda()
+    sparse(ids).sum().backward()
+    assert sparse.weight.grad.is_sparse

@@ -1724,6 +1724,115 @@ def add_rms_norm(res, delta, weight, eps: float = 1e-6, out_dtype=None):
 
 
 # ---------------------------------------------------------------------------------------------
+# log probabilities of given tokens
+# ---------------------------------------------------------------------------------------------
+def _logit_rows(t: torch.Tensor):
+    """(t, row pitch): t as rows of t.shape[-1] contiguous elements one pitch apart, at any address; copied where its strides
+    allow no such view."""
+    V = t.shape[-1]
+    if t.is_contiguous():
+        return t, V
+    lead = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    ld = lead[-1][1] if lead else V
+    if t.stride(-1) != 1 or ld < V or any(a[1] != b[0] * b[1] for a, b in zip(lead, lead[1:])):
+        return t.contiguous(), V
+    return t, ld
+
+
+@_operator("hawk_b200::token_logprobs_fwd", mutates_args=())
+def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int
+                       ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(logprob, entropy, top_logprobs, top_ids, stats) of token_logprobs; stats [.., 2] is what the backward needs."""
+    _same_device(logits, tokens)
+    lib = _lib.load()
+    x, ld = _logit_rows(logits)
+    tokens = tokens.contiguous()
+    V, rows, dev = x.shape[-1], tokens.numel(), x.device
+    assert x.shape[:-1] == tokens.shape
+    both = torch.empty((2, *tokens.shape), dtype=torch.float32, device=dev)
+    stats = torch.empty((*tokens.shape, 2), dtype=torch.float32, device=dev)
+    top_lp = torch.empty((*tokens.shape, top), dtype=torch.float32, device=dev)
+    top_id = torch.empty((*tokens.shape, top), dtype=torch.int64, device=dev)
+    lp, ent = both.unbind()
+    if rows:
+        with _on(x, "token_logprobs", 1):
+            _lib.check(lib.hawk_token_logprobs(x.data_ptr(), ld, tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), stats.data_ptr(),
+                                               top_lp.data_ptr() if top else None, top_id.data_ptr() if top else None, rows, V, top,
+                                               _dt(x), _stream(x)), "hawk_token_logprobs")
+    return lp, ent, top_lp, top_id, stats
+
+
+@token_logprobs_fwd.register_fake
+def _(logits, tokens, top):
+    f = lambda *tail, dtype=torch.float32: logits.new_empty((*tokens.shape, *tail), dtype=dtype)  # noqa: E731
+    return f(), f(), f(top), f(top, dtype=torch.int64), f(2)
+
+
+@_operator("hawk_b200::token_logprobs_bwd", mutates_args=())
+def token_logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
+                       g_logprob: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor]) -> torch.Tensor:
+    """The gradient of token_logprobs' logits."""
+    _same_device(logits, tokens, stats, logprob, entropy, g_logprob, g_entropy)
+    lib = _lib.load()
+    x, ld = _logit_rows(logits)
+    tokens = tokens.contiguous()
+    gl, ge = (None if g is None else g.float().contiguous() for g in (g_logprob, g_entropy))
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if dx.numel():
+        with _on(x, "token_logprobs_bwd", 1):
+            _lib.check(lib.hawk_token_logprobs_bwd(x.data_ptr(), ld, tokens.data_ptr(), stats.data_ptr(), logprob.data_ptr(),
+                                                   entropy.data_ptr(), _ptr(gl), _ptr(ge), dx.data_ptr(), tokens.numel(), x.shape[-1],
+                                                   _dt(x), _stream(x)), "hawk_token_logprobs_bwd")
+    return dx
+
+
+@token_logprobs_bwd.register_fake
+def _(logits, tokens, stats, logprob, entropy, g_logprob, g_entropy):
+    return logits.new_empty(logits.shape)
+
+
+def _tlp_setup(ctx, inputs, output):
+    logits, tokens, _ = inputs
+    lp, ent, top_lp, top_id, stats = output
+    ctx.save_for_backward(logits, tokens, stats, lp, ent)
+    ctx.mark_non_differentiable(top_lp, top_id, stats)
+    ctx.set_materialize_grads(False)
+
+
+def _tlp_backward(ctx, g_lp, g_ent, *_):
+    if g_lp is None and g_ent is None:
+        return None, None, None
+    return token_logprobs_bwd(*ctx.saved_tensors, g_lp, g_ent), None, None
+
+
+token_logprobs_fwd.register_autograd(_tlp_backward, setup_context=_tlp_setup)
+
+
+def _token_ids(tokens, shape):
+    if tokens.shape != shape:
+        raise ValueError(f"hawk_b200: tokens of shape {tuple(tokens.shape)} for rows of shape {tuple(shape)}")
+    if tokens.dtype == torch.int64:
+        return tokens
+    if tokens.dtype.is_floating_point or tokens.dtype.is_complex or tokens.dtype == torch.bool:
+        raise TypeError(f"hawk_b200: token ids are integers, not {tokens.dtype}")
+    return tokens.long()
+
+
+def token_logprobs(logits, tokens, top: int = 0):
+    """(logprob, entropy, top_logprobs, top_ids) from logits [.., V] (fp32 or bf16) and tokens [..]: the log probability of each
+    row's token, the entropy of its distribution (both fp32, in nats) and its `top` (up to 32) most probable tokens with their log
+    probabilities, by falling logit and, among equals, rising id.  One read of the logits, fp32 arithmetic; logprob and entropy are
+    differentiable, the alternatives are not.  A negative token leaves its row out: 0 and 0, no gradient, alternatives -inf and -1,
+    whatever the row holds.  A token >= V gives NaN.  Logits of -inf are tokens that cannot come; a row of nothing else has log
+    probability -inf, entropy 0 and no gradient."""
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"hawk_b200: logits of shape {tuple(logits.shape)}")
+    if not 0 <= top <= min(32, logits.shape[-1]):
+        raise ValueError(f"hawk_b200: top = {top} (0 to 32, and no more than the {logits.shape[-1]} tokens there are)")
+    return token_logprobs_fwd(logits, _token_ids(tokens, logits.shape[:-1]), int(top))[:4]
+
+
+# ---------------------------------------------------------------------------------------------
 # embedding
 # ---------------------------------------------------------------------------------------------
 @_operator("hawk_b200::embedding_fwd", mutates_args=())

@@ -403,6 +403,21 @@ size_t hawk_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H);
 int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dweight, void* workspace, size_t workspace_bytes,
                        int64_t N, int64_t V, int64_t H, int64_t padding_idx, float scale, int dtype, void* stream);
 
+/* Log probability of a given token, entropy and the `top` most probable tokens of each row of logits [rows, V] (row pitch ld
+ * in elements, any address):  logprob = x_t - lse, entropy = lse - sum p x, both fp32; stats [rows, 2] fp32 is for the backward.
+ * top_logprob [rows, top] fp32 and top_id [rows, top] int64 hold the alternatives by falling logit, ties by rising index;
+ * 0 <= top <= min(32, V), NULL where 0.
+ * A negative token leaves its row out: 0, 0, alternatives -infinity and -1, a zero gradient, whatever the row holds.  A token
+ * >= V gives a NaN logprob (and gradient).  A row of nothing but -infinity: logprob -infinity, entropy 0, a zero gradient.
+ * A NaN (or +infinity) in a row makes its logprob and entropy NaN; NaNs are no alternatives (-infinity and -1 where too few
+ * numbers are left).  Backward: dlogits [rows, V] contiguous; g_logprob, g_entropy [rows] fp32, NULL = 0. */
+int hawk_token_logprobs(const void* logits, int64_t ld, const int64_t* tokens, float* logprob, float* entropy,
+                        float* stats, float* top_logprob, int64_t* top_id, int64_t rows, int64_t V, int top, int dtype,
+                        void* stream);
+int hawk_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* tokens, const float* stats,
+                            const float* logprob, const float* entropy, const float* g_logprob, const float* g_entropy,
+                            void* dlogits, int64_t rows, int64_t V, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -84,3 +84,26 @@ def test_embedding_refuses_cpu_tensors():
         embedding(torch.zeros(3, dtype=torch.int64), torch.ones(4, 8))
     with pytest.raises(TypeError, match="integers"):
         embedding(torch.zeros(3), torch.ones(4, 8))
+
+
+def test_token_logprobs_argument_validation():
+    lib = L.load()
+    p = ctypes.c_void_p(4096)
+    call = lambda x=p, ld=10, rows=4, V=10, top=3, best=p, dt=0: lib.hawk_token_logprobs(  # noqa: E731
+        x, ld, p, p, p, p, best, best, rows, V, top, dt, None)
+    assert call(x=None) == -1 and call(best=None) == -1
+    assert call(rows=0) == call(V=0, top=0) == call(ld=9) == call(top=11) == call(top=-1) == call(V=64, ld=64, top=33) == -2
+    assert call(rows=1 << 28) == call(V=1 << 28, ld=1 << 28) == -2
+    assert call(dt=3) == -3 and call(x=ctypes.c_void_p(4098)) == -4
+    back = lambda x=p, ld=10, rows=4, dx=p, dt=1: lib.hawk_token_logprobs_bwd(  # noqa: E731
+        x, ld, p, p, p, p, None, None, dx, rows, 10, dt, None)
+    assert back(x=None) == back(dx=None) == -1
+    assert back(ld=9) == back(rows=0) == -2 and back(dt=2) == -3 and back(dx=ctypes.c_void_p(4097)) == -4
+
+
+def test_token_logprobs_refuses_cpu_tensors():
+    from hawk_b200 import token_logprobs
+    with pytest.raises(RuntimeError, match="CUDA"):
+        token_logprobs(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 2)
+    with pytest.raises(ValueError, match="top"):
+        token_logprobs(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 9)

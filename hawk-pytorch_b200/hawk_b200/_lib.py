@@ -68,6 +68,12 @@ SIGNATURES = {
     "hawk_embedding_bwd": (c_int, [_P, _P, _P, _P, c_size_t, c_int64, c_int64, c_int64, c_int64, c_float, c_int, _P]),
     "hawk_token_logprobs": (c_int, [_P, c_int64] + [_P] * 6 + [c_int64, c_int64, c_int, c_int, _P]),
     "hawk_token_logprobs_bwd": (c_int, [_P, c_int64] + [_P] * 7 + [c_int64, c_int64, c_int, _P]),
+    "hawk_linear_logprobs_saved_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
+    "hawk_linear_logprobs_scratch_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
+    "hawk_linear_logprobs_kernels": (c_int, [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int]),
+    "hawk_linear_logprobs": (c_int, [_P] * 6 + [c_size_t, c_int64, c_int64, c_int64, c_int, c_int, c_int, _P, _P]),
+    "hawk_linear_logprobs_bwd": (c_int, [_P] * 4 + [c_size_t] + [_P] * 5 + [c_int, _P, c_int, _P, c_size_t, c_int64, c_int64, c_int64,
+                                         c_int, c_int, _P, _P]),
     "hawk_scale": (c_int, [_P, _P, _P, c_int64, c_int, _P]),
     "hawk_cast_f32_bf16": (c_int, [_P, _P, c_int64, _P]),
     "hawk_gelu_mul_fwd": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, c_int, c_int, _P]),

@@ -13,12 +13,14 @@ from typing import List, Optional
 
 import torch
 
+from . import ops
 from .model import HawkModel, RNNCache
 
 
 class GraphedDecoder:
     """`prefill(ids)` runs the prompt eagerly and fills the caches; `step(token_ids)` replays the
-    captured single-token step and returns logits [B, 1, V] (a static buffer, overwritten per call)."""
+    captured single-token step and returns logits [B, 1, V] (a static buffer, overwritten per call); `logprobs(tokens)` says how
+    probable the tokens chosen from the latest logits were, and what else was."""
 
     def __init__(self, model: HawkModel, batch_size: int, cache_dtype: torch.dtype = torch.bfloat16,
                  autocast: bool = True, use_graph: bool = True):
@@ -32,6 +34,7 @@ class GraphedDecoder:
         self._ids = torch.zeros(batch_size, 1, dtype=torch.int64, device=self.device)
         self._logits: Optional[torch.Tensor] = None
         self._graph: Optional[torch.cuda.CUDAGraph] = None
+        self._latest: Optional[torch.Tensor] = None
 
     def _forward(self, ids):
         with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16, enabled=self.autocast):
@@ -42,7 +45,8 @@ class GraphedDecoder:
         assert ids.shape[0] == self.batch_size
         for c in self.caches:
             c.current_cache_size = 0
-        return self._forward(ids)
+        self._latest = self._forward(ids)
+        return self._latest
 
     def _capture(self):
         # warm up on a side stream (library handles, autotuning, allocator pools), keeping the cache
@@ -64,9 +68,18 @@ class GraphedDecoder:
     def step(self, token_ids: torch.Tensor) -> torch.Tensor:
         assert all(c.current_cache_size > 0 for c in self.caches), "call prefill() first"
         if not self.use_graph:
-            return self._forward(token_ids)
+            self._latest = self._forward(token_ids)
+            return self._latest
         if self._graph is None:
             self._capture()
         self._ids.copy_(token_ids)
         self._graph.replay()
-        return self._logits
+        self._latest = self._logits
+        return self._latest
+
+    def logprobs(self, tokens: torch.Tensor, top: int = 0):
+        """(logprob, entropy, top_logprobs, top_ids) of `tokens` ([B] or [B, 1]) under the logits that the latest `prefill` (its last
+        position) or `step` returned, as `ops.token_logprobs` gives them; a negative token leaves its sequence out."""
+        assert self._latest is not None, "call prefill() first"
+        with torch.no_grad():
+            return ops.token_logprobs(self._latest[:, -1], tokens.view(self.batch_size), top)

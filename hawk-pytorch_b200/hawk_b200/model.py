@@ -457,9 +457,8 @@ class HawkModel(nn.Module):
         return [RNNCache(self.config.recurrent_size, device, self.config.conv_width, batch_size, dtype)
                 for _ in self.layers]
 
-    def forward(self, input_ids, labels=None, layer_past: Optional[List[Optional[RNNCache]]] = None):
-        if layer_past is None:
-            layer_past = [None] * len(self.layers)
+    def _trunk(self, input_ids, layer_past: List[Optional[RNNCache]]):
+        """(residual stream, branch output not yet added to it, caches, whether the last layer ran as a chain)."""
         hidden = self.embed_tokens(input_ids)
         pending = None  # branch output not yet added to the residual stream: folded into the next norm
         caches = []
@@ -470,6 +469,34 @@ class HawkModel(nn.Module):
             chained = done is not None
             hidden, pending, cache = (*done, past) if chained else layer.step(hidden, pending, past)
             caches.append(cache)
+        return hidden, pending, caches, chained
+
+    @staticmethod
+    def _without_last(hidden):
+        """The activations that predict a next token (hawk/hawk.py:291-300), [N,H]."""
+        if (hidden.is_cuda and hidden.dim() == 3 and hidden.shape[1] >= 2 and hidden.numel() and hidden.is_contiguous()
+                and hidden.shape[2] * hidden.element_size() % 16 == 0 and not torch.compiler.is_compiling()):
+            return ops.drop_last(hidden).view(-1, hidden.shape[-1])
+        return hidden[..., :-1, :].reshape(-1, hidden.shape[-1])
+
+    def token_logprobs(self, input_ids, labels=None):
+        """(logprob, entropy), fp32 [B,T-1]: of labels[:, t+1] (`labels` as in `forward`, input_ids by default) given the tokens up
+        to position t, and of the distribution it is drawn from.  A negative label leaves its position out: 0, 0 and no gradient
+        (the padding of a ragged batch).  Differentiable, e.g. for policy-gradient losses; for scoring call it under no_grad.  The
+        logits are never in memory (`ops.linear_logprobs`)."""
+        if self.use_cache:
+            raise ValueError("token_logprobs runs whole sequences: construct the model without use_cache, or use "
+                             "GraphedDecoder.logprobs")
+        labels = input_ids if labels is None else labels
+        hidden, pending, _, _ = self._trunk(input_ids, [None] * len(self.layers))
+        _, hidden = self.norm.add_forward(hidden, pending)
+        lp, entropy = ops.linear_logprobs(self.lm_head.weight, self._without_last(hidden), labels[..., 1:].reshape(-1))
+        return lp.view(labels[..., 1:].shape), entropy.view(labels[..., 1:].shape)
+
+    def forward(self, input_ids, labels=None, layer_past: Optional[List[Optional[RNNCache]]] = None):
+        if layer_past is None:
+            layer_past = [None] * len(self.layers)
+        hidden, pending, caches, chained = self._trunk(input_ids, layer_past)
         if self.use_cache and pending is not None and pending.dtype == torch.bfloat16:
             autocast = _chain_ok(hidden)
             if autocast is not None and _plain(self.norm, RMSNorm) and _plain(self.lm_head, nn.Linear):
@@ -483,13 +510,8 @@ class HawkModel(nn.Module):
         if labels is None:
             return self.lm_head(hidden)
         # next-token loss: position t predicts token t+1 (hawk/hawk.py:291-300)
-        if (hidden.is_cuda and hidden.dim() == 3 and hidden.shape[1] >= 2 and hidden.numel() and hidden.is_contiguous()
-                and hidden.shape[2] * hidden.element_size() % 16 == 0 and not torch.compiler.is_compiling()):
-            act = ops.drop_last(hidden).view(-1, hidden.shape[-1])
-        else:
-            act = hidden[..., :-1, :].reshape(-1, hidden.shape[-1])
         targets = labels[..., 1:].reshape(-1)
-        return ops.fused_cross_entropy(self.lm_head.weight, act, targets)
+        return ops.fused_cross_entropy(self.lm_head.weight, self._without_last(hidden), targets)
 
 
 # the configurations named by the benchmark contract

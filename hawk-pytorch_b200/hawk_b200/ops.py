@@ -1832,6 +1832,98 @@ def token_logprobs(logits, tokens, top: int = 0):
     return token_logprobs_fwd(logits, _token_ids(tokens, logits.shape[:-1]), int(top))[:4]
 
 
+# the same from activations and the head's weight, without logits in memory
+@_operator("hawk_b200::linear_logprobs_fwd", mutates_args=())
+def linear_logprobs_fwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.Tensor, want_grad: bool
+                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(logprob, entropy, saved) of linear_logprobs; with want_grad `saved` holds what linear_logprobs_bwd needs."""
+    _same_device(weight, act, tokens)
+    lib = _lib.load()
+    weight, act, tokens = _dense16(weight), _dense16(act), tokens.contiguous()
+    (V, H), N, dev = weight.shape, tokens.numel(), act.device
+    assert act.shape == (*tokens.shape, H)
+    lp, ent = torch.empty((2, *tokens.shape), dtype=torch.float32, device=dev).unbind()
+    saved = torch.empty(lib.hawk_linear_logprobs_saved_bytes(N, H, V, _dt(weight), _dt(act), int(want_grad)), dtype=torch.uint8, device=dev)
+    if N:
+        with _on(act, "linear_logprobs", lambda: lib.hawk_linear_logprobs_kernels(N, H, V, _dt(weight), _dt(act), 0, 0)):
+            _lib.check(lib.hawk_linear_logprobs(weight.data_ptr(), act.data_ptr(), tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(),
+                                                saved.data_ptr(), saved.numel(), N, H, V, _dt(weight), _dt(act), int(want_grad),
+                                                _status_word(dev).data_ptr(), _stream(act)), "hawk_linear_logprobs")
+    return lp, ent, saved
+
+
+@linear_logprobs_fwd.register_fake
+def _(weight, act, tokens, want_grad):
+    (V, H), N = weight.shape, tokens.numel()
+    up = lambda n: (n + 255) // 256 * 256  # noqa: E731
+    n = up(N * ((V + 127) // 128) * 16) + up(N * 8) + up(N * 4) + (up(N * ((V + 7) // 8 * 8) * 2) if want_grad else 0)
+    n += up(V * H * 2) if weight.dtype == torch.float32 else 0
+    n += up(N * H * 2) if act.dtype == torch.float32 else 0
+    out = act.new_empty((2, *tokens.shape), dtype=torch.float32)
+    return out[0].clone(), out[1].clone(), act.new_empty(n, dtype=torch.uint8)
+
+
+@_operator("hawk_b200::linear_logprobs_bwd", mutates_args=())
+def linear_logprobs_bwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.Tensor, saved: torch.Tensor, logprob: torch.Tensor,
+                        entropy: torch.Tensor, g_logprob: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor], want_dw: bool,
+                        want_da: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(d weight, d act) in the operands' dtypes (empty where not wanted)."""
+    _same_device(weight, act, tokens, saved, logprob, entropy, g_logprob, g_entropy)
+    lib = _lib.load()
+    weight, act, tokens = _dense16(weight), _dense16(act), tokens.contiguous()
+    (V, H), N, dev = weight.shape, tokens.numel(), act.device
+    dw = torch.empty(weight.shape if want_dw else 0, dtype=weight.dtype, device=dev)
+    da = torch.empty(act.shape if want_da else 0, dtype=act.dtype, device=dev)
+    if N == 0:
+        return dw.zero_(), da
+    gl, ge = (None if g is None else g.float().contiguous() for g in (g_logprob, g_entropy))
+    ws = torch.empty(lib.hawk_linear_logprobs_scratch_bytes(N, H, V, _dt(act), int(want_dw), int(want_da)), dtype=torch.uint8, device=dev)
+    with _on(act, "linear_logprobs_bwd",
+             lambda: lib.hawk_linear_logprobs_kernels(N, H, V, _dt(weight), _dt(act), int(want_dw), int(want_da))):
+        _lib.check(lib.hawk_linear_logprobs_bwd(weight.data_ptr(), act.data_ptr(), tokens.data_ptr(), saved.data_ptr(), saved.numel(),
+                                                logprob.data_ptr(), entropy.data_ptr(), _ptr(gl), _ptr(ge), dw.data_ptr() if want_dw else None,
+                                                _dt(dw), da.data_ptr() if want_da else None, _dt(da), ws.data_ptr(), ws.numel(), N, H, V,
+                                                _dt(weight), _dt(act), _status_word(dev).data_ptr(), _stream(act)),
+                   "hawk_linear_logprobs_bwd")
+    return dw, da
+
+
+@linear_logprobs_bwd.register_fake
+def _(weight, act, tokens, saved, logprob, entropy, g_logprob, g_entropy, want_dw, want_da):
+    return weight.new_empty(weight.shape if want_dw else 0), act.new_empty(act.shape if want_da else 0)
+
+
+def _llp_setup(ctx, inputs, output):
+    weight, act, tokens, _ = inputs
+    lp, ent, saved = output
+    ctx.save_for_backward(weight, act, tokens, saved, lp, ent)
+    ctx.mark_non_differentiable(saved)
+    ctx.set_materialize_grads(False)
+
+
+def _llp_backward(ctx, g_lp, g_ent, _):
+    want = ctx.needs_input_grad[:2]
+    if (g_lp is None and g_ent is None) or not any(want):
+        return None, None, None, None
+    dw, da = linear_logprobs_bwd(*ctx.saved_tensors, g_lp, g_ent, *want)
+    return dw if want[0] else None, da if want[1] else None, None, None
+
+
+linear_logprobs_fwd.register_autograd(_llp_backward, setup_context=_llp_setup)
+
+
+def linear_logprobs(weight, act, tokens):
+    """(logprob, entropy) of `tokens` [..] under the distributions softmax(act @ weight.T): weight [V,H], act [..,H] (fp32 or bf16, H
+    a multiple of 8), both results fp32 of tokens' shape and differentiable in weight and act.  What fused_cross_entropy is to the
+    mean loss: bf16 tensor-core products (operands in fp32 are rounded, as there), but the logits stay unrounded fp32 sums and are
+    never in memory; a forward that waits for its backward holds N * V bf16 values.  Negative tokens and those >= V as in
+    token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold."""
+    if weight.dim() != 2 or act.dim() < 1 or act.shape[-1] != weight.shape[1]:
+        raise ValueError(f"hawk_b200: activations of shape {tuple(act.shape)} with a weight of shape {tuple(weight.shape)}")
+    want = torch.is_grad_enabled() and (weight.requires_grad or act.requires_grad)
+    return linear_logprobs_fwd(weight, act, _token_ids(tokens, act.shape[:-1]), want)[:2]
+
+
 # ---------------------------------------------------------------------------------------------
 # embedding
 # ---------------------------------------------------------------------------------------------

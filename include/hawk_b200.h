@@ -418,6 +418,24 @@ int hawk_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* token
                             const float* logprob, const float* entropy, const float* g_logprob, const float* g_entropy,
                             void* dlogits, int64_t rows, int64_t V, int dtype, void* stream);
 
+/* hawk_token_logprobs of x = act . weight^T (act [N,H], weight [V,H], H a multiple of 8) without alternatives, and without logits
+ * in memory: bf16 operands (fp32 ones are rounded, as hawk_linear_ce_fwd does), fp32 sums, unrounded logits.  Negative tokens and
+ * those >= V as there.  `saved` (256-byte aligned, hawk_linear_logprobs_saved_bytes) holds what the backward needs if want_grad
+ * (then N*V bf16 values among it); the backward leaves it as it is.  Gradients in dw_dtype / da_dtype, either may be NULL;
+ * g_logprob, g_entropy [N] fp32, NULL = 0.  A left-out row has no part in dweight, whatever act holds there.
+ * hawk_linear_logprobs_kernels: the forward's launches (want_dw = want_da = 0) or the backward's. */
+size_t hawk_linear_logprobs_saved_bytes(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_grad);
+size_t hawk_linear_logprobs_scratch_bytes(int64_t N, int64_t H, int64_t V, int a_dtype, int want_dw, int want_da);
+int hawk_linear_logprobs_kernels(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_dw, int want_da);
+int hawk_linear_logprobs(const void* weight, const void* act, const int64_t* tokens, float* logprob, float* entropy,
+                         void* saved, size_t saved_bytes, int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype,
+                         int want_grad, int* status, void* stream);
+int hawk_linear_logprobs_bwd(const void* weight, const void* act, const int64_t* tokens, const void* saved,
+                             size_t saved_bytes, const float* logprob, const float* entropy, const float* g_logprob,
+                             const float* g_entropy, void* dweight, int dw_dtype, void* dact, int da_dtype, void* scratch,
+                             size_t scratch_bytes, int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int* status,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif

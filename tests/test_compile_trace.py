@@ -54,3 +54,14 @@ def test_fused_operator_functions_trace(monkeypatch):
     for fused in (False, True):  # the recurrent core with the cuBLAS form and with the fused gate kernels
         monkeypatch.setattr(ops, "gates_kernel_ok", lambda x_, nb, bw, f=fused: f)
         _trace(lambda a: ops.recurrent_core(a, cw, cb, wx, wa, gb, lam)[0].float().sum(), xy)
+
+
+def test_end_operators_trace():
+    from hawk_b200 import ops
+    w, ids = torch.randn(32, 64, requires_grad=True), torch.randint(0, 32, (5, 7))
+    targets = _trace(lambda i, w: ops.embedding(i, w, 2.0, 3), ids, w)
+    assert any("embedding_fwd" in t for t in targets)
+    targets = _trace(lambda x, t: ops.token_logprobs(x, t, 2), torch.randn(5, 7, 32, requires_grad=True), ids)
+    assert any("token_logprobs_fwd" in t for t in targets)
+    targets = _trace(ops.linear_logprobs, w, torch.randn(5, 7, 64, requires_grad=True), ids)
+    assert any("linear_logprobs_fwd" in t for t in targets)

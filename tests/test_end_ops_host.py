@@ -107,3 +107,27 @@ def test_token_logprobs_refuses_cpu_tensors():
         token_logprobs(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 2)
     with pytest.raises(ValueError, match="top"):
         token_logprobs(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), 9)
+
+
+def test_linear_logprobs_argument_validation():
+    lib = L.load()
+    p = ctypes.c_void_p(4096)
+    saved = lib.hawk_linear_logprobs_saved_bytes(4, 64, 300, 0, 1, 1)
+    assert saved >= 300 * 64 * 2 + 4 * 304 * 2 + 4 * 3 * 16 and lib.hawk_linear_logprobs_saved_bytes(4, 64, 300, 1, 1, 0) < saved
+    fwd = lambda w=p, sv=p, n=saved, N=4, H=64, dt=0, st=p: lib.hawk_linear_logprobs(  # noqa: E731
+        w, p, p, p, p, sv, n, N, H, 300, dt, 1, 1, st, None)
+    assert fwd(w=None) == fwd(st=None) == -1 and fwd(N=0) == fwd(H=60) == -2 and fwd(dt=4) == -3
+    assert fwd(sv=None) == fwd(n=saved - 1) == -5 and fwd(w=ctypes.c_void_p(4104)) == -4
+    scratch = lib.hawk_linear_logprobs_scratch_bytes(4, 64, 300, 1, 1, 1)
+    bwd = lambda dw=p, sc=p, n=scratch, sv=saved, H=64: lib.hawk_linear_logprobs_bwd(  # noqa: E731
+        p, p, p, p, sv, p, p, None, None, dw, 0, None, 0, sc, n, 4, H, 300, 0, 1, p, None)
+    assert bwd(dw=None) == -1 and bwd(H=4) == -2 and bwd(sc=None) == bwd(sv=saved - 1) == -5 and bwd(dw=ctypes.c_void_p(4100)) == -4
+    need = lib.hawk_linear_logprobs_scratch_bytes(4, 64, 300, 1, 1, 0)
+    assert bwd(n=need - 1) == -5
+    assert lib.hawk_linear_logprobs_kernels(4, 64, 300, 0, 1, 0, 0) == 3
+
+
+def test_linear_logprobs_refuses_cpu_tensors():
+    from hawk_b200 import linear_logprobs
+    with pytest.raises(RuntimeError, match="CUDA"):
+        linear_logprobs(torch.zeros(9, 8), torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64))

@@ -5,7 +5,10 @@
 //      gradient is wanted it stores e, in bf16: at most 1, so its rounding is 2^-9 of a probability whatever the logits' size
 //      (a bf16 logit of 20 is off by 0.06, 6 % of its probability), and exactly 1 at each group's maximum, so that the
 //      probability of a token that all but certain is as exact as the sums.
-//   2. reduce  a warp per row over its groups: m, log s, log probability and entropy.
+//   2. reduce  a warp per row over its groups: m, log s, log probability and entropy.  The token's own logit is formed once more,
+//      as a plain fp32 dot product: the tensor core truncates its running sum at every step of 16 products, which leaves a large
+//      logit a little too small (2e-5 of 16 after 2048 products), and a log probability near 0 would be nothing but that.  The
+//      sums get its term anew as well.  N rows of act and weight read: 50 us of 11 ms at N32760 H2048 V32000.
 // Backward, from e and the groups' maxima (2 N V bytes kept instead of a third GEMM: forming the logits again takes 2 N H V
 // flops, 3.1 ms at N32760 H2048 V32000 where writing and reading e takes 1):
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
@@ -18,11 +21,25 @@ namespace hawk {
 
 __global__ void __launch_bounds__(256)
 score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ correct, const int64_t* __restrict__ tokens,
-                    float* __restrict__ logprob, float* __restrict__ entropy, float2* __restrict__ stats, int N, int groups,
+                    const __nv_bfloat16* __restrict__ weight, const __nv_bfloat16* __restrict__ act, float* __restrict__ logprob,
+                    float* __restrict__ entropy, float2* __restrict__ stats, int N, int H, int V, int groups,
                     const int* __restrict__ status) {
   const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (row >= N) return;
   const float4* g = score + (long long)row * groups;
+  const int64_t token = tokens[row];
+  float own = 0.f;
+  if (token >= 0 && token < V) {
+    const __nv_bfloat16 *a = act + (long long)row * H, *w = weight + token * H;
+#pragma unroll 4
+    for (int i = lane * 8; i < H; i += 256) {
+      float av[8], wv[8];
+      VecIO<__nv_bfloat16, 8>::load(a + i, av);
+      VecIO<__nv_bfloat16, 8>::load(w + i, wv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) own = fmaf(av[j], wv[j], own);
+    }
+  }
   float m = -INFINITY;
   for (int i = lane; i < groups; i += 32) m = fmaxf(m, g[i].x);
 #pragma unroll
@@ -39,11 +56,20 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
   for (int o = 16; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     sx += __shfl_xor_sync(0xffffffffu, sx, o);
+    own += __shfl_xor_sync(0xffffffffu, own, o);
   }
   if (lane == 0) {
-    const float logs = logf(s), nan = __int_as_float(0x7fc00000);
-    float lp = (correct[row] - m) - logs, ent = logs - 0.6931471805599453f * sx / s;
-    if (tokens[row] < 0) lp = ent = 0.f;
+    const float nan = __int_as_float(0x7fc00000);
+    if (token >= 0 && token < V) {
+      const float t0 = (correct[row] - m) * kLog2e, t1 = (own - m) * kLog2e, e0 = ex2_approx(t0), e1 = ex2_approx(t1);
+      s = (s - e0) + e1;
+      sx = (sx - e0 * t0) + e1 * t1;
+    } else {
+      own = nan;
+    }
+    const float logs = logf(s);
+    float lp = (own - m) - logs, ent = logs - 0.6931471805599453f * sx / s;
+    if (token < 0) lp = ent = 0.f;
     if (*status != 0) lp = ent = nan;  // a GEMM gave up a wait (this call's, or an earlier one nobody has looked at)
     logprob[row] = lp;
     entropy[row] = ent;
@@ -218,8 +244,9 @@ extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const i
   else
     rc = launch_gemm<EPI_SCORE, 1, false, false>(ab, H, wb, H, nullptr, false, S.ldV, (int)N, (int)V, (int)H, 1, ep, status, st);
   if (rc != HAWK_OK) return rc;
-  score_reduce_kernel<<<(unsigned)((N + 7) / 8), 256, 0, st>>>(ep.score, correct, tokens, logprob, entropy,
-                                                               reinterpret_cast<float2*>(sv + S.stats), (int)N, S.groups, status);
+  score_reduce_kernel<<<(unsigned)((N + 7) / 8), 256, 0, st>>>(ep.score, correct, tokens, wb, ab, logprob, entropy,
+                                                               reinterpret_cast<float2*>(sv + S.stats), (int)N, (int)H, (int)V, S.groups,
+                                                               status);
   return launch_status();
 }
 

@@ -40,7 +40,8 @@ struct Cand {
 __device__ __forceinline__ bool comes_before(const Cand& a, const Cand& b) { return a.x > b.x || (a.x == b.x && a.j < b.j); }
 
 struct LpShared {  // what the blocks of a cluster read of one another
-  float m, s, sx;  // maximum, sum of e^(x - m), sum of e^(x - m) (x - m) log2 e
+  float m, s, sx;  // maximum, sum of e^(x - m) over the other elements, sum of e^(x - m) (x - m) log2 e
+  float ties;      // elements at the maximum
   int found;
   Cand best[kLpMaxTop];
 };
@@ -147,7 +148,7 @@ template <typename T, int NV, bool LONG>
 __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
   constexpr int N = RowVec<T>::N;
   __shared__ LpShared sh;
-  __shared__ float red[3][kLpWarps], subset[kLpSubsets];
+  __shared__ float red[4][kLpWarps], subset[kLpSubsets];
   __shared__ Cand cand[kLpCand], draw[kLpWarps];
   __shared__ int ncand;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -200,8 +201,9 @@ __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
   __syncthreads();
   const float m = warp_max(lane < kLpWarps ? red[0][lane] : -INFINITY);
 
-  // 2. the sums.  Where m is -infinity no number is here: there is nothing to add, but a NaN (which no maximum shows) is to be seen
-  float s = 0.f, sx = 0.f;
+  // 2. the sums, of the terms below 1 alone: log s = log1p of them is then as exact for a token that is all but certain (s = 1.001)
+  // as for any other.  Only threads that hold a maximum have to look for it.  Where m is -infinity no number is here: there is nothing to add, but a NaN (which no maximum shows) is to be seen
+  float s = 0.f, sx = 0.f, ties = 0.f;
   if (m == -INFINITY)
     each([&](int, uint4 raw) {
       float x[N];
@@ -209,6 +211,19 @@ __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (x[j] != x[j]) s = x[j];
+    });
+  else if (tmax == m)
+    each([&](int, uint4 raw) {
+      float x[N];
+      RowVec<T>::unpack(raw, x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        float t;
+        const float e = lp_exp(x[j] - m, t);
+        ties += x[j] == m ? 1.f : 0.f;
+        s += x[j] == m ? (t - t) : e;  // 0; NaN where m is infinite
+        sx = fmaf(e, t, sx);
+      }
     });
   else
     each([&](int, uint4 raw) {
@@ -224,9 +239,11 @@ __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
     });
   s = warp_sum(s);
   sx = warp_sum(sx);
+  ties = warp_sum(ties);
   if (lane == 0) {
     red[1][warp] = s;
     red[2][warp] = sx;
+    red[3][warp] = ties;
   }
 
   // 3. the alternatives among this block's elements, in order, to sh.best
@@ -305,18 +322,20 @@ __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
   }
   __syncthreads();
   if (warp == 0) {
-    const float bs = warp_sum(lane < kLpWarps ? red[1][lane] : 0.f), bx = warp_sum(lane < kLpWarps ? red[2][lane] : 0.f);
+    const float bs = warp_sum(lane < kLpWarps ? red[1][lane] : 0.f), bx = warp_sum(lane < kLpWarps ? red[2][lane] : 0.f),
+                bt = warp_sum(lane < kLpWarps ? red[3][lane] : 0.f);
     if (lane == 0) {
       sh.m = m;
       sh.s = bs;
       sh.sx = bx;
+      sh.ties = bt;
     }
   }
 
   // 4. the cluster's blocks together, in the first of them
   if (blocks > 1) lp_cluster_sync(); else __syncthreads();
   if (rank == 0) {
-    float M = -INFINITY, S = 0.f, SX = 0.f;
+    float M = -INFINITY, S = 0.f, SX = 0.f, ties = 0.f;  // S without the elements at the maximum
     for (uint32_t b = 0; b < blocks; ++b) M = fmaxf(M, __uint_as_float(lp_ld_remote(lp_remote(&sh.m, b))));
     for (uint32_t b = 0; b < blocks; ++b) {
       const float bm = __uint_as_float(lp_ld_remote(lp_remote(&sh.m, b))), bs = __uint_as_float(lp_ld_remote(lp_remote(&sh.s, b)));
@@ -325,11 +344,12 @@ __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
         continue;
       }
       float t;
-      const float k = lp_exp(bm - M, t);
-      S = fmaf(bs, k, S);
-      SX = fmaf(fmaf(bs, t, __uint_as_float(lp_ld_remote(lp_remote(&sh.sx, b)))), k, SX);  // terms move by (m_b - M) log2 e
+      const float k = lp_exp(bm - M, t), bt = __uint_as_float(lp_ld_remote(lp_remote(&sh.ties, b))), ball = bs + bt;
+      if (bm == M) ties += bt;
+      S = fmaf(bm == M ? bs : ball, k, S);
+      SX = fmaf(fmaf(ball, t, __uint_as_float(lp_ld_remote(lp_remote(&sh.sx, b)))), k, SX);  // terms move by (m_b - M) log2 e
     }
-    const float logs = logf(S);
+    const float logs = log1pf((ties - 1.f) + S);  // no element at a maximum: -infinity of 0, or NaN
     if (tid == 0) {
       const float x = token < a.V ? to_float(row.p[token]) : __int_as_float(0x7fc00000);
       if (M == -INFINITY && S == 0.f) {  // nothing but -infinity: no distribution
@@ -337,7 +357,7 @@ __global__ void __launch_bounds__(kLpThreads, 2) lp_rows_kernel(LpArgs a) {
         a.entropy[r] = 0.f;
       } else {
         a.logprob[r] = (x - M) - logs;
-        a.entropy[r] = logs - kLn2 * SX / S;
+        a.entropy[r] = logs - kLn2 * SX / (S + ties);
       }
       a.stats[2 * r] = M;
       a.stats[2 * r + 1] = logs;

@@ -8,15 +8,16 @@
 namespace hawk {
 
 struct AdamwArgs {
-  float lr, beta1, beta2, eps, decay_factor;  // decay_factor = 1 - lr * weight_decay
+  float beta1, beta2, new1, new2;             // new = 1 - beta
+  float eps, decay_factor;                    // decay_factor = 1 - lr * weight_decay
   float step_size;                            // lr / (1 - beta1^t)
   float inv_sqrt_bc2;                         // 1 / sqrt(1 - beta2^t)
 };
 
 __device__ __forceinline__ float adamw_one(float p, float g, float& m, float& v, const AdamwArgs& a) {
   p *= a.decay_factor;
-  m = fmaf(a.beta1, m, (1.f - a.beta1) * g);
-  v = fmaf(a.beta2, v, (1.f - a.beta2) * g * g);
+  m = fmaf(a.beta1, m, a.new1 * g);
+  v = fmaf(a.beta2, v, a.new2 * g * g);
   const float denom = fmaf(sqrtf(v), a.inv_sqrt_bc2, a.eps);
   return p - a.step_size * (m / denom);
 }
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__(256) adamw_kernel(const __grid_constant__ Adam
 
 using namespace hawk;
 
-extern "C" int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2,
+extern "C" int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, double beta1, double beta2,
                                        float eps, float weight_decay, int64_t step, const float* grad_scale, void* stream) {
   HAWK_REQUIRE(tensors, HAWK_ERR_NULL);
   HAWK_REQUIRE(aligned(grad_scale, 4), HAWK_ERR_ALIGN);
@@ -94,12 +95,13 @@ extern "C" int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int cou
     HAWK_REQUIRE(aligned(t.p, 4) && aligned(t.g, 4) && aligned(t.m, 4) && aligned(t.v, 4) && aligned(t.p_bf16, 2), HAWK_ERR_ALIGN);
   }
   AdamwArgs a;
-  a.lr = lr;
-  a.beta1 = beta1;
-  a.beta2 = beta2;
+  a.beta1 = (float)beta1;
+  a.beta2 = (float)beta2;
+  a.new1 = (float)(1.0 - beta1);  // 1 - 0.999 from the fp32 rounding of 0.999 is 1.3e-5 off
+  a.new2 = (float)(1.0 - beta2);
   a.eps = eps;
   a.decay_factor = 1.f - lr * weight_decay;
-  const double bc1 = 1.0 - pow((double)beta1, (double)step), bc2 = 1.0 - pow((double)beta2, (double)step);
+  const double bc1 = 1.0 - pow(beta1, (double)step), bc2 = 1.0 - pow(beta2, (double)step);
   a.step_size = (float)((double)lr / bc1);
   a.inv_sqrt_bc2 = (float)(1.0 / sqrt(bc2));
   for (int i0 = 0; i0 < count;) {

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_int64, c_longlong, c_size_t, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int64, c_longlong, c_size_t, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhawk_b200.so")
@@ -59,7 +59,7 @@ SIGNATURES = {
     "hawk_decode_norm_linear": (c_int, [_P, _P, _P, c_float, _P, _P, _P, c_size_t] + [c_int] * 6 + [_P, _P]),
     "hawk_adamw_step": (c_int, [_P, _P, _P, _P, _P, c_int64, c_float, c_float, c_float, c_float, c_float, c_int64, _P]),
     "hawk_adamw_multi": (c_int, [c_char_p, c_int, c_float, c_float, c_float, c_float, c_float, c_int64, _P]),
-    "hawk_adamw_multi_scaled": (c_int, [c_char_p, c_int, c_float, c_float, c_float, c_float, c_float, c_int64, _P, _P]),
+    "hawk_adamw_multi_scaled": (c_int, [c_char_p, c_int, c_float, c_double, c_double, c_float, c_float, c_int64, _P, _P]),
     "hawk_grad_norm_workspace_bytes": (c_size_t, [c_int]),
     "hawk_grad_norm": (c_int, [c_char_p, c_int, c_float, _P, _P, c_size_t, _P]),
     "hawk_scale_multi": (c_int, [c_char_p, c_int, _P, _P]),

@@ -373,8 +373,9 @@ typedef struct hawk_adamw_tensor {
 } hawk_adamw_tensor;
 int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
                      float weight_decay, int64_t step, void* stream);
-/* The same with the gradients taken times *grad_scale (a device scalar, e.g. the second result of hawk_grad_norm; NULL = 1). */
-int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
+/* The same with the gradients taken times *grad_scale (a device scalar, e.g. the second result of hawk_grad_norm; NULL = 1).
+ * The betas are doubles: 1 - beta, formed from a beta rounded to fp32, would be 1.3e-5 off at 0.999. */
+int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, double beta1, double beta2, float eps,
                             float weight_decay, int64_t step, const float* grad_scale, void* stream);
 
 /* The 2-norm over all elements of `count` tensors (a host array, n >= 1 contiguous elements each, fp32 or bf16), and the

@@ -5,14 +5,17 @@
 // N rows read and V rows written, the rows that no token names among them.
 //
 // Backward, three launches:
-//   1. group   positions in the order of their ids (a stable counting sort).  A block owns a slice of the vocabulary and
-//              reads all ids (they come from L2: 148 blocks x 8 B, against rows of kilobytes): it counts those below its slice,
-//              which gives its place in the result without a word from the other blocks, and queues its own in shared memory
-//              in their order; one warp then hands out the places, 32 at a time (match.any ranks equal ids).
-//   2. windows sums of 32 consecutive sorted positions, only for windows that lie inside the run of an id with more than 64
-//              of them: the most frequent token of a text is 5 to 10 % of it, and one warp would walk its rows alone.
-//   3. rows    a warp per table row and 512 columns (fp32: 4 16-byte loads in flight per position, 4 positions at a time): its
-//              few positions, or for the long runs the ragged ends and the windows' sums; zeros where there are none.
+//   1. group   the positions of each id side by side, in their order (a stable counting sort).  Block b owns the ids that are b
+//              modulo the number of blocks (the frequent tokens of a vocabulary have low ids: by ranges, the first of 148 blocks had
+//              half of a text's tokens, 143 us of a 30 us kernel's work at 32768 tokens) and reads all ids (from L2: 128 blocks x
+//              8 B, against rows of kilobytes): it counts those of the blocks before it, which gives its place in the result
+//              without a word from them, and queues its own in shared memory in their order.  The queue's warps rank equal ids
+//              among their 32 (match.any) and take turns at the counters.
+//   2. windows sums of 16 consecutive places, only for windows inside the run of an id with more than 32 of them: the most
+//              frequent token of a text is 5 to 10 % of it, and one warp would walk its rows alone.
+//   3. rows    a warp per 8 table rows and 512 columns walks the places of its rows as one stream, three rows of dout ahead
+//              whichever table rows they belong to (most have no position or one: a loop per row would wait for each); zeros where
+//              there is nothing.  Long runs it passes over: the first blocks add them up from the windows' sums and ragged ends.
 #include <algorithm>
 
 #include "common.cuh"
@@ -57,9 +60,27 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int64_t* __restric
 }
 
 // ---- backward 1: positions grouped by id ---------------------------------------------------------------------
+// Where the positions of id v come in the order of the groups: those of block v mod 2^log_blocks together, and there the ids whose
+// quotients lie slots / 8 apart next to one another, so that the 8 table rows of a warp are one that may be frequent and 7 rarer ones
+// (8 neighbouring quotients: the first warp had 8 rows of 60 positions each to add, 158 us where 60 were left to do).
+constexpr int kRowGroup = 8;
+struct EmbedOrder {
+  int log_blocks, slots;  // slots: ids of a block, a multiple of kRowGroup
+  __host__ __device__ int64_t groups() const { return (int64_t)slots << log_blocks; }
+  __device__ int slot(int64_t v) const {  // within its block
+    const int x = (int)(v >> log_blocks), q = slots / kRowGroup;
+    return x % q * kRowGroup + x / q;
+  }
+  __device__ int64_t place(int64_t v) const { return (v & ((1 << log_blocks) - 1)) * slots + slot(v); }
+  __device__ int64_t id(int64_t place) const {  // the inverse
+    const int64_t block = place / slots, s = place % slots;
+    return (s % kRowGroup * (slots / kRowGroup) + s / kRowGroup) << log_blocks | block;
+  }
+};
 constexpr int kGroupThreads = 1024, kIdsPerThread = 8, kGroupStep = kGroupThreads * kIdsPerThread;
 constexpr int kQueue = kGroupStep;  // one step's ids always fit
-constexpr int kMaxSlice = 4096;
+constexpr int kMaxSlots = 4096, kMinLogBlocks = 7;
+constexpr int kWindow = 16, kLong = 2 * kWindow;  // a run of more than kLong positions holds a whole window
 
 // exclusive sum over the block's threads; `all`: of all of them.  The shared words may be reused after the next barrier.
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& all) {
@@ -83,243 +104,330 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& all) {
   return inc - v + (warp > 0 ? before : 0);
 }
 
-// One step's ids of this thread (its 8 positions are consecutive, so the threads are in the order of the positions): which of
-// them are in [lo, hi), and how many valid ones lie below.
+// One step's ids of this thread: its 8 positions are consecutive, so the threads are in the order of the positions.
 struct StepIds {
   int64_t id[kIdsPerThread];
-  uint32_t mine;
+  __device__ __forceinline__ void load(const int64_t* ids, int64_t i0, int64_t N) {
+    if (i0 + kIdsPerThread <= N && aligned16(ids)) {  // i0 is a multiple of 8
+#pragma unroll
+      for (int q = 0; q < kIdsPerThread / 2; ++q) {
+        const longlong2 t = __ldg(reinterpret_cast<const longlong2*>(ids + i0) + q);
+        id[2 * q] = t.x;
+        id[2 * q + 1] = t.y;
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < kIdsPerThread; ++q) id[q] = i0 + q < N ? __ldg(ids + i0 + q) : -1;
+    }
+  }
+  // which of them are this block's; `below` counts those of the blocks before it
+  __device__ __forceinline__ uint32_t mine(int64_t V, int64_t padding, int log_blocks, int block, int& below) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int q = 0; q < kIdsPerThread; ++q) {
+      if (id[q] < 0 || id[q] >= V || id[q] == padding) continue;
+      const int b = (int)id[q] & ((1 << log_blocks) - 1);
+      below += b < block;
+      if (b == block) m |= 1u << q;
+    }
+    return m;
+  }
 };
-__device__ __forceinline__ void load_step(const int64_t* ids, int64_t i0, int64_t N, int64_t lo, int64_t hi, int64_t padding, StepIds& s,
-                                          int& below) {
-  if (i0 + kIdsPerThread <= N && aligned16(ids)) {  // i0 is a multiple of 8
-#pragma unroll
-    for (int q = 0; q < kIdsPerThread / 2; ++q) {
-      const longlong2 t = __ldg(reinterpret_cast<const longlong2*>(ids + i0) + q);
-      s.id[2 * q] = t.x;
-      s.id[2 * q + 1] = t.y;
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < kIdsPerThread; ++q) s.id[q] = i0 + q < N ? __ldg(ids + i0 + q) : -1;
-  }
-  s.mine = 0;
-#pragma unroll
-  for (int q = 0; q < kIdsPerThread; ++q) {
-    const int64_t id = s.id[q];
-    if (id < 0 || id == padding) continue;
-    below += id < lo;
-    if (id >= lo && id < hi) s.mine |= 1u << q;
-  }
-}
 
-__device__ __forceinline__ void place(const uint2* queue, int n, int* cursor, int* perm) {  // one warp
-  const int lane = threadIdx.x & 31;
-  for (int k = 0; k < n; k += 32) {
-    const bool have = k + lane < n;
+// hands out the places of n <= kQueue queued (slot, position) pairs; the whole block
+__device__ __forceinline__ void place(const uint2* queue, int n, int* cursor, int* perm) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int k = 0; k < n; k += kGroupThreads) {
+    const int i = k + threadIdx.x, warps = min(kGroupThreads / 32, (n - k + 31) / 32);
+    const bool have = i < n;
     const uint32_t active = __ballot_sync(0xffffffffu, have);
+    uint2 q = make_uint2(0u, 0u);
+    uint32_t peers = 0;
     if (have) {
-      const uint2 q = queue[k + lane];
-      const uint32_t peers = __match_any_sync(active, q.x);
-      const int rank = __popc(peers & ((1u << lane) - 1)), at = cursor[q.x];
-      perm[at + rank] = (int)q.y;
-      __syncwarp(active);
-      if (rank == 0) cursor[q.x] = at + __popc(peers);
+      q = queue[i];
+      peers = __match_any_sync(active, q.x);
     }
-    __syncwarp();
+    const int rank = __popc(peers & ((1u << lane) - 1));
+    int at = 0;
+    for (int w = 0; w < warps; ++w) {  // in the order of the positions
+      if (w == warp && have) {
+        at = cursor[q.x];
+        __syncwarp(active);
+        if (rank == 0) cursor[q.x] = at + __popc(peers);
+      }
+      __syncthreads();
+    }
+    if (have) perm[at + rank] = (int)q.y;
   }
 }
 
 __global__ void __launch_bounds__(kGroupThreads) embed_group_kernel(const int64_t* __restrict__ ids, int64_t N, int64_t V, int64_t padding,
-                                                                    int slice, int* __restrict__ perm, int* __restrict__ start) {
+                                                                    EmbedOrder order, int* __restrict__ perm, int* __restrict__ start,
+                                                                    int* __restrict__ owner, int windows) {
   extern __shared__ uint2 queue[];                       // [kQueue]
-  int* count = reinterpret_cast<int*>(queue + kQueue);   // [slice], the cursors later
+  int* count = reinterpret_cast<int*>(queue + kQueue);   // [slots], the cursors later
   __shared__ int warp_sums[2][32];
-  const int tid = threadIdx.x;
-  const int64_t lo = (int64_t)blockIdx.x * slice, hi = lo + slice < V ? lo + slice : V;
-  for (int j = tid; j < slice; j += kGroupThreads) count[j] = 0;
+  const int tid = threadIdx.x, slots = order.slots, log_blocks = order.log_blocks;
+  for (int j = tid; j < slots; j += kGroupThreads) count[j] = 0;
+  int below = 0, total = 0, all, step = 0;
+  StepIds s, next;
+  s.load(ids, tid * kIdsPerThread, N);
   __syncthreads();
-  int below = 0, total = 0, all;
-  StepIds s;
-  int step = 0;
   for (int64_t base = 0; base < N; base += kGroupStep, step ^= 1) {  // the scans take turns with their shared words
     const int64_t i0 = base + tid * kIdsPerThread;
-    load_step(ids, i0, N, lo, hi, padding, s, below);
-    int at = total + block_scan(__popc(s.mine), warp_sums[step], all);
+    if (base + kGroupStep < N) next.load(ids, i0 + kGroupStep, N);
+    const uint32_t mine = s.mine(V, padding, log_blocks, blockIdx.x, below);
+    int at = total + block_scan(__popc(mine), warp_sums[step], all);
 #pragma unroll
     for (int q = 0; q < kIdsPerThread; ++q)
-      if (s.mine >> q & 1) {
-        const int j = (int)(s.id[q] - lo);
+      if (mine >> q & 1) {
+        const int j = order.slot(s.id[q]);
         atomicAdd(&count[j], 1);
         if (at < kQueue) queue[at] = make_uint2((uint32_t)j, (uint32_t)(i0 + q));
         ++at;
       }
     total += all;
+    s = next;
   }
   __syncthreads();
   int ahead;
   block_scan(below, warp_sums[0], ahead);
   __syncthreads();
   // counts -> first places
-  constexpr int kPer = kMaxSlice / kGroupThreads;
+  constexpr int kPer = kMaxSlots / kGroupThreads;
   int c[kPer], sum = 0;
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
     const int j = tid * kPer + q;
-    c[q] = j < slice ? count[j] : 0;
+    c[q] = j < slots ? count[j] : 0;
     sum += c[q];
   }
   int at = ahead + block_scan(sum, warp_sums[1], all);
+  int* mystart = start + (int64_t)blockIdx.x * slots;
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
     const int j = tid * kPer + q;
-    if (j < slice) {
-      count[j] = at;
-      if (lo + j < V) start[lo + j] = at;
-    }
+    if (j < slots) count[j] = mystart[j] = at;
     at += c[q];
   }
-  if (hi == V && tid == 0) start[V] = ahead + total;
+  const int behind = ahead + total;
+  if (blockIdx.x == gridDim.x - 1 && tid == 0) mystart[slots] = behind;
+  __syncthreads();
+  // whose long run each window lies in (-1: none): the windows that start in this block's share, and those behind the last share
+  const int w_end = blockIdx.x == gridDim.x - 1 ? windows : min(windows, (behind + kWindow - 1) / kWindow);
+  for (int w = (ahead + kWindow - 1) / kWindow + tid; w < w_end; w += kGroupThreads) {
+    int lo = 0, hi = slots;  // the last slot that starts at or before the window
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (count[mid] <= w * kWindow) lo = mid; else hi = mid;
+    }
+    const int end = lo + 1 < slots ? count[lo + 1] : behind;
+    owner[w] = end - count[lo] > kLong && (w + 1) * kWindow <= end ? (int)(blockIdx.x * slots + lo) : -1;
+  }
   __syncthreads();
   if (total <= kQueue) {
-    if (tid < 32) place(queue, total, count, perm);
+    place(queue, total, count, perm);
     return;
   }
   for (int64_t base = 0; base < N; base += kGroupStep, step ^= 1) {  // more than the queue holds: read the ids again
     const int64_t i0 = base + tid * kIdsPerThread;
-    load_step(ids, i0, N, lo, hi, padding, s, below);
-    int to = block_scan(__popc(s.mine), warp_sums[step], all);
+    s.load(ids, i0, N);
+    const uint32_t mine = s.mine(V, padding, log_blocks, blockIdx.x, below);
+    int to = block_scan(__popc(mine), warp_sums[step], all);
 #pragma unroll
     for (int q = 0; q < kIdsPerThread; ++q)
-      if (s.mine >> q & 1) queue[to++] = make_uint2((uint32_t)(s.id[q] - lo), (uint32_t)(i0 + q));
+      if (mine >> q & 1) queue[to++] = make_uint2((uint32_t)order.slot(s.id[q]), (uint32_t)(i0 + q));
     __syncthreads();
-    if (tid < 32) place(queue, all, count, perm);
+    place(queue, all, count, perm);
     __syncthreads();
   }
 }
 
 // ---- backward 2 and 3: sums --------------------------------------------------------------------------------
-constexpr int kWindow = 32, kLong = 2 * kWindow;  // a run of more than kLong positions holds a whole window
 
 template <typename T>
 __host__ __device__ constexpr int unit_vectors(int vec) { return vec == 1 ? 8 : 512 / (32 * vec); }  // vectors per lane: 512 columns (256 in the scalar form)
 
-// acc += the rows of `src` at the given places, one after the other; four rows in flight
-template <typename T, int VEC, int U, typename Row>
-__device__ __forceinline__ void add_rows(float (&acc)[U][VEC], const T* src, int H, int c0, int s, int e, Row row) {
-  int i = s;
-  for (; i + 4 <= e; i += 4) {
-    float v[4][U][VEC];
+// a warp per window and 32 * VEC columns, all of its rows in flight
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) embed_window_kernel(const T* __restrict__ dout, const int* perm, const int* owner, float* partial, int H,
+                                                           int narrow, int64_t units) {
+  pdl_wait();
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  const int lane = threadIdx.x & 31, win = (int)(unit / narrow), c0 = ((int)(unit % narrow) * 32 + lane) * VEC;
+  if (owner[win] < 0) return;
+  const int mine = perm[win * kWindow + lane % kWindow];
+  float v[kWindow][VEC], acc[VEC];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const T* p = src + (int64_t)row(i + r) * H + c0;
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (c0 + u * 32 * VEC < H) VecIO<T, VEC>::load(p + u * 32 * VEC, v[r][u]);
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (c0 + u * 32 * VEC < H)
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[u][j] += v[r][u][j];
+  for (int r = 0; r < kWindow; ++r) {
+    const int64_t p = __shfl_sync(0xffffffffu, mine, r);
+    if (c0 < H) VecIO<T, VEC>::load(dout + p * H + c0, v[r]);
   }
-  for (; i < e; ++i) {
-    const T* p = src + (int64_t)row(i) * H + c0;
-    float v[U][VEC];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * 32 * VEC < H) VecIO<T, VEC>::load(p + u * 32 * VEC, v[u]);
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + u * 32 * VEC < H)
+  for (int r = 0; r < kWindow; ++r)
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[u][j] += v[u][j];
+    for (int j = 0; j < VEC; ++j) acc[j] += v[r][j];
+  if (c0 < H) VecIO<float, VEC>::store(partial + (int64_t)win * H + c0, acc);
+}
+
+// acc += n rows of `src`, the k-th of them row(k), one after the other; 32 values per lane in flight
+template <typename T, int VEC, typename Row>
+__device__ __forceinline__ void add_rows(float (&acc)[VEC], const T* src, int H, int c0, int n, Row row) {
+  constexpr int D = VEC == 1 ? 16 : 32 / VEC;
+#pragma unroll 1
+  for (int k = 0; k < n; k += D) {
+    float v[D][VEC];
+#pragma unroll
+    for (int r = 0; r < D; ++r)
+      if (k + r < n) VecIO<T, VEC>::load(src + (int64_t)row(k + r) * H + c0, v[r]);
+#pragma unroll
+    for (int r = 0; r < D; ++r)
+      if (k + r < n) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += v[r][j];
+      }
   }
 }
 
+// the row of an id with a long run, by the units of its first window: 32 * VEC columns of the ragged ends, then of the windows' sums
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embed_window_kernel(const int64_t* __restrict__ ids, const T* __restrict__ dout,
-                                                           const int* __restrict__ perm, const int* __restrict__ start,
-                                                           float* __restrict__ partial, int64_t V, int H, int chunks, int64_t units) {
-  constexpr int U = unit_vectors<T>(VEC);
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= units) return;
-  const int win = (int)(unit / chunks), c0 = ((int)(unit % chunks) * 32 * U + (threadIdx.x & 31)) * VEC;
-  const int s = win * kWindow;
-  if (s + kWindow > start[V]) return;
-  const int64_t id = ids[perm[s]];
-  if (ids[perm[s + kWindow - 1]] != id || start[id + 1] - start[id] <= kLong) return;
-  float acc[U][VEC];
+__device__ __forceinline__ void long_run(const T* dout, const int* perm, const int* start, const float* partial, const int* owner, T* dw,
+                                         EmbedOrder order, int H, float scale, int narrow, int64_t unit) {
+  const int win = (int)(unit / narrow), k = owner[win], c0 = ((int)(unit % narrow) * 32 + (threadIdx.x & 31)) * VEC;
+  if (k < 0 || c0 >= H) return;
+  const int s = start[k], e = start[k + 1], w1 = e / kWindow, head = win * kWindow - s, tail = e - w1 * kWindow;
+  if (head >= kWindow) return;
+  float acc[VEC];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+  add_rows<T, VEC>(acc, dout, H, c0, head + tail, [&](int i) { return perm[i < head ? s + i : w1 * kWindow + i - head]; });
+  add_rows<float, VEC>(acc, partial, H, c0, w1 - win, [&](int i) { return win + i; });
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
-  add_rows<T, VEC, U>(acc, dout, H, c0, s, s + kWindow, [&](int i) { return perm[i]; });
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (c0 + u * 32 * VEC < H)
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) partial[(int64_t)win * H + c0 + u * 32 * VEC + j] = acc[u][j];
+  for (int j = 0; j < VEC; ++j) acc[j] *= scale;
+  VecIO<T, VEC>::store(dw + order.id(k) * H + c0, acc);
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embed_rows_kernel(const T* __restrict__ dout, const int* __restrict__ perm,
-                                                         const int* __restrict__ start, const float* __restrict__ partial,
-                                                         T* __restrict__ dw, int H, float scale, int chunks, int64_t units) {
+__global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict__ dout, const int* perm, const int* start, const float* partial,
+                                                         const int* owner, T* __restrict__ dw, EmbedOrder order, int64_t V, int H,
+                                                         float scale, int chunks, int64_t units, int narrow, int64_t long_units) {
   constexpr int U = unit_vectors<T>(VEC);
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit < long_units) {  // long runs first: they take longest
+    long_run<T, VEC>(dout, perm, start, partial, owner, dw, order, H, scale, narrow, unit);
+    return;
+  }
+  unit -= long_units;
   if (unit >= units) return;
-  const int64_t v = unit / chunks;
-  const int c0 = ((int)(unit % chunks) * 32 * U + (threadIdx.x & 31)) * VEC;
-  const int s = start[v], e = start[v + 1];
+  const int lane = threadIdx.x & 31;
+  const int64_t k0 = unit / chunks * kRowGroup;
+  const int c0 = ((int)(unit % chunks) * 32 * U + lane) * VEC;
+  const int64_t id0 = order.id(k0), apart = (int64_t)(order.slots / kRowGroup) << order.log_blocks;
+  const int st = start[k0 + min(lane, kRowGroup)];
+  const int first = __shfl_sync(0xffffffffu, st, 0), last = __shfl_sync(0xffffffffu, st, kRowGroup);
   float acc[U][VEC];
+  const auto clear = [&] {
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
-  const auto at = [&](int i) { return perm[i]; };
-  if (e - s <= kLong) {
-    add_rows<T, VEC, U>(acc, dout, H, c0, s, e, at);
-  } else {
-    const int w0 = (s + kWindow - 1) / kWindow, w1 = e / kWindow;
-    add_rows<T, VEC, U>(acc, dout, H, c0, s, w0 * kWindow, at);
-    for (int w = w0; w < w1; ++w)
+      for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
+  };
+  const auto write = [&](int row) {
+    const int64_t v = id0 + row * apart;
+    if (v >= V) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * 32 * VEC < H) {
+        float o[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = acc[u][j] * scale;
+        VecIO<T, VEC>::store(dw + v * H + c0 + u * 32 * VEC, o);
+      }
+  };
+  // the places of all rows as one stream, three rows of dout ahead; long runs are passed over
+  float v0[U][VEC], v1[U][VEC], v2[U][VEC];
+  int pbase = first, places = first + lane < last ? perm[first + lane] : 0;  // 32 places, one per lane
+  int i = first, ahead = first, bound = first, row = -1;  // v2, v1, v0 hold places ahead - 1, - 2, - 3
+  uint32_t runs = 0;                                      // rows that are long runs
+  clear();
+#pragma unroll 1
+  for (;;) {
+#pragma unroll 1
+    while (i == bound) {  // the row ends here (and any empty ones behind it)
+      if (row >= 0 && !(runs >> row & 1)) {
+        write(row);
+        clear();
+      }
+      if (++row == kRowGroup) break;
+      bound = __shfl_sync(0xffffffffu, st, row + 1);
+      if (bound - i > kLong) {
+        runs |= 1u << row;
+        i = ahead = bound;
+      }
+    }
+    if (row == kRowGroup) break;
+#pragma unroll 1
+    do {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (c0 + u * 32 * VEC < H)
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) acc[u][j] += partial[(int64_t)w * H + c0 + u * 32 * VEC + j];
-    add_rows<T, VEC, U>(acc, dout, H, c0, w1 * kWindow, e, at);
+        for (int j = 0; j < VEC; ++j) {
+          v0[u][j] = v1[u][j];
+          v1[u][j] = v2[u][j];
+        }
+      if (ahead < last) {
+        if (ahead - pbase >= 32) {
+          pbase = ahead;
+          places = ahead + lane < last ? perm[ahead + lane] : 0;
+        }
+        const T* p = dout + (int64_t)__shfl_sync(0xffffffffu, places, ahead - pbase) * H + c0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (c0 + u * 32 * VEC < H) VecIO<T, VEC>::load(p + u * 32 * VEC, v2[u]);
+      }
+      ++ahead;
+    } while (ahead - 3 < i);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[u][j] += v0[u][j];
+    ++i;
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (c0 + u * 32 * VEC < H) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[u][j] *= scale;
-      VecIO<T, VEC>::store(dw + v * H + c0 + u * 32 * VEC, acc[u]);
-    }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct EmbedWs {
-  size_t perm, start, partial, total;
+  size_t perm, start, partial, owner, total;
 };
+// as many blocks as nearly fill the GPU, more where a block's counters would not fit its shared memory
+static EmbedOrder embed_order(int64_t V) {
+  EmbedOrder o{kMinLogBlocks, 0};
+  while ((V >> o.log_blocks) >= kMaxSlots) ++o.log_blocks;
+  const int64_t slots = (V + (1LL << o.log_blocks) - 1) >> o.log_blocks;
+  o.slots = (int)((slots + kRowGroup - 1) / kRowGroup * kRowGroup);
+  return o;
+}
+
 static EmbedWs embed_ws(int64_t N, int64_t V, int64_t H) {
   EmbedWs L;
   size_t o = 0;
   L.perm = o;    o += up256((size_t)N * 4);
-  L.start = o;   o += up256((size_t)(V + 1) * 4);
+  L.start = o;   o += up256((size_t)(embed_order(V).groups() + 1) * 4);
   L.partial = o; o += N > kLong ? up256((size_t)(N / kWindow) * H * 4) : 0;
+  L.owner = o;   o += N > kLong ? up256((size_t)(N / kWindow) * 4) : 0;
   L.total = o;
   return L;
 }
 
 static int check_embed(int64_t N, int64_t V, int64_t H, int dtype) {
   HAWK_REQUIRE(valid_dtype(dtype), HAWK_ERR_DTYPE);
-  HAWK_REQUIRE(N >= 1 && N < (1LL << 31) - kGroupStep && V >= 1 && V < (1LL << 31) - kMaxSlice && H >= 1 && H < (1 << 24), HAWK_ERR_SHAPE);
+  HAWK_REQUIRE(N >= 1 && N < (1LL << 31) - kGroupStep && V >= 1 && V < (1LL << 30) && H >= 1 && H < (1 << 24), HAWK_ERR_SHAPE);
   return HAWK_OK;
 }
 
@@ -341,20 +449,19 @@ static int embed_fwd(const int64_t* ids, const void* w, void* out, int64_t N, in
 }
 
 template <typename T, int VEC>
-static int embed_sums(const int64_t* ids, const void* dout, void* dw, const int* perm, const int* start, float* partial, int64_t N,
-                      int64_t V, int H, float scale, cudaStream_t st) {
-  const int cols = 32 * VEC * unit_vectors<T>(VEC), chunks = (H + cols - 1) / cols;
-  const int64_t windows = N > kLong ? N / kWindow * chunks : 0, rows = V * chunks;
-  HAWK_REQUIRE((rows + 7) / 8 < (1LL << 31) && (windows + 7) / 8 < (1LL << 31), HAWK_ERR_SHAPE);
+static int embed_sums(const void* dout, void* dw, const int* perm, const int* start, float* partial, const int* owner, EmbedOrder order,
+                      int64_t N, int64_t V, int H, float scale, cudaStream_t st) {
+  const int cols = 32 * VEC * unit_vectors<T>(VEC), chunks = (H + cols - 1) / cols, narrow = (H + 32 * VEC - 1) / (32 * VEC);
+  const int64_t windows = N > kLong ? N / kWindow * narrow : 0, rows = order.groups() / kRowGroup * chunks;
+  HAWK_REQUIRE((rows + windows + 7) / 8 < (1LL << 31), HAWK_ERR_SHAPE);
+  const auto* g = static_cast<const T*>(dout);
   if (windows) {
-    embed_window_kernel<T, VEC><<<(unsigned)((windows + 7) / 8), 256, 0, st>>>(ids, static_cast<const T*>(dout), perm, start, partial, V, H,
-                                                                               chunks, windows);
-    const int rc = launch_status();
+    const int rc = launch_kernel(embed_window_kernel<T, VEC>, dim3((unsigned)((windows + 7) / 8)), dim3(256), 0, st, true, 1, g, perm, owner,
+                                 partial, H, narrow, windows);
     if (rc != HAWK_OK) return rc;
   }
-  embed_rows_kernel<T, VEC><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(static_cast<const T*>(dout), perm, start, partial,
-                                                                        static_cast<T*>(dw), H, scale, chunks, rows);
-  return launch_status();
+  return launch_kernel(embed_rows_kernel<T, VEC>, dim3((unsigned)((rows + windows + 7) / 8)), dim3(256), 0, st, true, 1, g, perm, start,
+                       partial, owner, static_cast<T*>(dw), order, V, H, scale, chunks, rows, narrow, windows);
 }
 
 #define HAWK_BY_VEC(f, dtype, vec, ...)                                                                      \
@@ -394,17 +501,18 @@ extern "C" int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dw
   auto* ws = static_cast<unsigned char*>(workspace);
   auto* perm = reinterpret_cast<int*>(ws + L.perm);
   auto* start = reinterpret_cast<int*>(ws + L.start);
-  // a slice of the vocabulary for every SM; no narrower than a warp's worth
-  const int slice = (int)std::min<int64_t>(kMaxSlice, std::max<int64_t>(32, (V + 147) / 148));
-  const size_t smem = kQueue * sizeof(uint2) + (size_t)slice * sizeof(int);
+  auto* owner = reinterpret_cast<int*>(ws + L.owner);
+  const int windows = N > kLong ? (int)(N / kWindow) : 0;
+  const EmbedOrder order = embed_order(V);
+  const size_t smem = kQueue * sizeof(uint2) + (size_t)order.slots * sizeof(int);
   if (cudaFuncSetAttribute(embed_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
     (void)cudaGetLastError();
     return HAWK_ERR_LAUNCH;
   }
-  embed_group_kernel<<<(unsigned)((V + slice - 1) / slice), kGroupThreads, smem, st>>>(ids, N, V, padding_idx, slice, perm, start);
+  embed_group_kernel<<<1u << order.log_blocks, kGroupThreads, smem, st>>>(ids, N, V, padding_idx, order, perm, start, owner, windows);
   const int rc = launch_status();
   if (rc != HAWK_OK) return rc;
   const int vec = common_vec((int)H, es, dout, dweight);
-  return HAWK_BY_VEC(embed_sums, dtype, vec, ids, dout, dweight, perm, start, reinterpret_cast<float*>(ws + L.partial), N, V, (int)H, scale,
-                     st);
+  return HAWK_BY_VEC(embed_sums, dtype, vec, dout, dweight, perm, start, reinterpret_cast<float*>(ws + L.partial),
+                     owner, order, N, V, (int)H, scale, st);
 }

@@ -46,13 +46,13 @@ def test_embedding_matches(n, V, H, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("n", [63, 64, 65, 96, 97, 8191, 8192, 8193, 40000])
+@pytest.mark.parametrize("n", [16, 31, 32, 33, 47, 48, 49, 63, 64, 65, 96, 97, 8191, 8192, 8193, 40000])
 def test_one_token_everywhere(n, dtype):
     """All positions of one block's slice, past its queue; runs that end inside, at and after a window."""
     _check(torch.full((n,), 11, device="cuda"), 40, 72, dtype)
 
 
-@pytest.mark.parametrize("lead", [0, 1, 31, 32, 33, 63])
+@pytest.mark.parametrize("lead", [0, 1, 15, 16, 17, 31, 32, 33, 63])
 def test_runs_across_windows(lead):
     ids = torch.cat([torch.zeros(lead, dtype=torch.int64), torch.full((200,), 5), torch.full((64,), 6), torch.full((65,), 8),
                      torch.arange(9, 30)]).cuda()
@@ -168,7 +168,7 @@ def test_module_and_model():
         model(ids, ids).backward()
     counts = dict(ops.LOG.counts)
     ops.LOG.enabled = False
-    assert counts["embedding_fwd"] == 1 and counts["embedding_bwd"] == 2
+    assert counts["embedding_fwd"] == 1 and counts["embedding_bwd"] == 3  # 45 tokens: with the long runs' launch
     cpu = M.Embedding(50, 24, scale=2.0)
     assert torch.equal(cpu(ids.cpu()), 2.0 * cpu.weight[ids.cpu()])
     sparse = M.Embedding(50, 24, sparse=True).cuda()

@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import inspect
 import math
-import struct
+from array import array
 from typing import Optional, Tuple
 
 import torch
@@ -1747,13 +1747,13 @@ def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int
     lib = _lib.load()
     x, ld = _logit_rows(logits)
     tokens = tokens.contiguous()
-    V, rows, dev = x.shape[-1], tokens.numel(), x.device
-    assert x.shape[:-1] == tokens.shape
-    both = torch.empty((2, *tokens.shape), dtype=torch.float32, device=dev)
-    stats = torch.empty((*tokens.shape, 2), dtype=torch.float32, device=dev)
-    top_lp = torch.empty((*tokens.shape, top), dtype=torch.float32, device=dev)
-    top_id = torch.empty((*tokens.shape, top), dtype=torch.int64, device=dev)
-    lp, ent = both.unbind()
+    V, rows, shape = x.shape[-1], tokens.numel(), tokens.shape
+    assert x.shape[:-1] == shape
+    lp = torch.empty_like(tokens, dtype=torch.float32)
+    ent = torch.empty_like(lp)
+    stats = torch.empty((*shape, 2), dtype=torch.float32, device=x.device)
+    top_lp = torch.empty((*shape, top), dtype=torch.float32, device=x.device)
+    top_id = torch.empty_like(top_lp, dtype=torch.int64)
     if rows:
         with _on(x, "token_logprobs", 1):
             _lib.check(lib.hawk_token_logprobs(x.data_ptr(), ld, tokens.data_ptr(), lp.data_ptr(), ent.data_ptr(), stats.data_ptr(),
@@ -1842,7 +1842,8 @@ def linear_logprobs_fwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.T
     weight, act, tokens = _dense16(weight), _dense16(act), tokens.contiguous()
     (V, H), N, dev = weight.shape, tokens.numel(), act.device
     assert act.shape == (*tokens.shape, H)
-    lp, ent = torch.empty((2, *tokens.shape), dtype=torch.float32, device=dev).unbind()
+    lp = torch.empty_like(tokens, dtype=torch.float32)
+    ent = torch.empty_like(lp)
     saved = torch.empty(lib.hawk_linear_logprobs_saved_bytes(N, H, V, _dt(weight), _dt(act), int(want_grad)), dtype=torch.uint8, device=dev)
     if N:
         with _on(act, "linear_logprobs", lambda: lib.hawk_linear_logprobs_kernels(N, H, V, _dt(weight), _dt(act), 0, 0)):
@@ -1859,8 +1860,7 @@ def _(weight, act, tokens, want_grad):
     n = up(N * ((V + 127) // 128) * 16) + up(N * 8) + up(N * 4) + (up(N * ((V + 7) // 8 * 8) * 2) if want_grad else 0)
     n += up(V * H * 2) if weight.dtype == torch.float32 else 0
     n += up(N * H * 2) if act.dtype == torch.float32 else 0
-    out = act.new_empty((2, *tokens.shape), dtype=torch.float32)
-    return out[0].clone(), out[1].clone(), act.new_empty(n, dtype=torch.uint8)
+    return (*(act.new_empty(tokens.shape, dtype=torch.float32) for _ in range(2)), act.new_empty(n, dtype=torch.uint8))
 
 
 @_operator("hawk_b200::linear_logprobs_bwd", mutates_args=())
@@ -2018,26 +2018,37 @@ def embedding(ids, weight, scale: float = 1.0, padding_idx: Optional[int] = None
 # ---------------------------------------------------------------------------------------------
 # the norm of a model's gradients
 # ---------------------------------------------------------------------------------------------
+_tensor = torch.Tensor
+_DT_ALL = frozenset(_DT)
+
+
 def _norm_table(tensors):
-    """(hawk_norm_tensor's of the tensors that hold anything, their device, what has to stay alive until the call is made)"""
-    flat, keep, device = [], [], None
-    for t in tensors:
-        if not t.is_cuda:
-            raise RuntimeError("hawk_b200: tensors must be on a CUDA device (there is no CPU path)")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise RuntimeError(f"hawk_b200: tensors on {device} and {t.device} in one call")
-        if t.layout != torch.strided:
-            raise TypeError(f"hawk_b200: a {t.layout} tensor in a norm")
-        n = t.numel()
-        if n == 0:
-            continue
-        if not t.is_contiguous():
-            t = t.contiguous()
-            keep.append(t)
-        flat += (t.data_ptr(), n, _dt(t))
-    return flat, device, keep
+    """(hawk_norm_tensor's of the tensors that hold anything, their device, what has to stay alive until the call is made).  The
+    properties are asked for all tensors at a time: 107 tensors took 51 us in a loop, of the 36 that their norm takes on the GPU."""
+    tensors = list(tensors)
+    if not tensors:
+        return array("q"), None, tensors
+    index = set(map(_tensor.get_device, tensors))
+    if len(index) > 1 or -1 in index:
+        for t in tensors:
+            if not t.is_cuda:
+                raise RuntimeError("hawk_b200: tensors must be on a CUDA device (there is no CPU path)")
+        _same_device(*tensors)
+    dtypes = list(map(_tensor.dtype.__get__, tensors))
+    if not _DT_ALL.issuperset(dtypes):
+        for t in tensors:
+            _dt(t)
+    if not all(map(_tensor.is_contiguous, tensors)):  # raises for layouts other than strided
+        tensors = [t.contiguous() for t in tensors]
+    counts = list(map(_tensor.numel, tensors))
+    if 0 in counts:
+        full = [i for i, n in enumerate(counts) if n]
+        tensors, dtypes, counts = ([v[i] for i in full] for v in (tensors, dtypes, counts))
+    table = array("q", bytes(24 * len(tensors)))
+    table[0::3] = array("q", map(_tensor.data_ptr, tensors))
+    table[1::3] = array("q", counts)
+    table[2::3] = array("q", map(_DT.__getitem__, dtypes))
+    return table, torch.device("cuda", index.pop()), tensors
 
 
 def _grad_norm(table, device, max_norm: float) -> torch.Tensor:
@@ -2051,7 +2062,7 @@ def _grad_norm(table, device, max_norm: float) -> torch.Tensor:
     out = torch.empty(2, dtype=torch.float32, device=device)
     ws = torch.empty(lib.hawk_grad_norm_workspace_bytes(count), dtype=torch.uint8, device=device)
     with _on(out, "grad_norm", (count + 1023) // 1024 + 1):
-        _lib.check(lib.hawk_grad_norm(struct.pack(f"{len(table)}q", *table), count, max_norm, out.data_ptr(), ws.data_ptr(),
+        _lib.check(lib.hawk_grad_norm(table.tobytes(), count, max_norm, out.data_ptr(), ws.data_ptr(),
                                       ws.numel(), _stream(out)), "hawk_grad_norm")
     return out
 
@@ -2067,9 +2078,10 @@ def grad_norm(tensors) -> torch.Tensor:
 def scale_in_place(tensors, scale: torch.Tensor) -> None:
     """t *= scale for every t of `tensors` (fp32 or bf16, contiguous, not overlapping), with `scale` an fp32 scalar on their
     device; nothing is read or written where it is 1."""
-    table, device, keep = _norm_table(tensors)
-    if keep:
+    tensors = list(tensors)
+    if not all(map(_tensor.is_contiguous, tensors)):
         raise ValueError("hawk_b200: scale_in_place takes contiguous tensors")
+    table, device, keep = _norm_table(tensors)
     if not table:
         return
     spans = sorted((p, p + n * (2 if d == _lib.HAWK_BF16 else 4)) for p, n, d in zip(table[::3], table[1::3], table[2::3]))
@@ -2080,6 +2092,6 @@ def scale_in_place(tensors, scale: torch.Tensor) -> None:
     lib = _lib.load()
     count = len(table) // 3
     with _on(scale, "scale_multi", (count + 1023) // 1024):
-        _lib.check(lib.hawk_scale_multi(struct.pack(f"{len(table)}q", *table), count, scale.data_ptr(), _stream(scale)),
+        _lib.check(lib.hawk_scale_multi(table.tobytes(), count, scale.data_ptr(), _stream(scale)),
                    "hawk_scale_multi")
     torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])  # written behind autograd's back

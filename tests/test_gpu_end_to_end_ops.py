@@ -147,3 +147,32 @@ def test_scored_decoding(use_graph):
 def test_a_cached_model_refuses_whole_sequences():
     with pytest.raises(ValueError, match="use_cache"):
         _model(4, use_cache=True).token_logprobs(torch.zeros(1, 4, dtype=torch.int64, device="cuda"))
+
+
+def test_through_the_dispatcher():
+    """The same calls where torch has to see the operators: under a mode and a profiler, and as torch.library's checks want them."""
+    import hawk_b200 as h
+    from hawk_b200 import ops
+
+    class Passes(torch.overrides.TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(50, 64, generator=g, device="cuda").bfloat16().requires_grad_()
+    a = torch.randn(3, 7, 64, generator=g, device="cuda").bfloat16().requires_grad_()
+    x = torch.randn(3, 7, 50, generator=g, device="cuda").requires_grad_()
+    ids = torch.randint(-1, 50, (3, 7), generator=g, device="cuda")
+
+    def everything():
+        out = [h.embedding(ids.clamp(min=0), w, 2.0, 3), *h.linear_logprobs(w, a, ids), *h.token_logprobs(x, ids, 4)]
+        grads = torch.autograd.grad([o.float().sum() for o in out if o.requires_grad], [w, a, x])
+        return [*out, *grads]
+    direct = everything()
+    for context in (Passes, torch.profiler.profile):
+        with context():
+            seen = everything()
+        assert all(torch.equal(p, q) for p, q in zip(direct, seen))
+    tests = ("test_schema", "test_autograd_registration", "test_faketensor", "test_aot_dispatch_static")
+    torch.library.opcheck(ops.embedding_fwd, (ids.clamp(min=0), w, 2.0, 3), test_utils=tests)
+    torch.library.opcheck(ops.token_logprobs_fwd, (x, ids, 4), test_utils=tests)
+    torch.library.opcheck(ops.linear_logprobs_fwd, (w.detach(), a.detach(), ids, False), test_utils=tests[:1] + tests[2:3])

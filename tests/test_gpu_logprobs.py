@@ -75,7 +75,8 @@ def test_ties_and_order(V, dtype):
     """Rows whose candidates are many: all equal, rising, falling, two values, few distinct ones."""
     n = torch.arange(V, device="cuda")
     rows = [torch.zeros(V, device="cuda"), n / 64, -n / 64, (n % 7 == 3).float(), (n % 3).float() - 1, (n == V - 1).float() * 9,
-            torch.where(n < 40, 1.0, 1.0 + (n % 2) / 128), (n // 5 % 100).float()]
+            torch.where(n < 40, 1.0, 1.0 + (n % 2) / 128), (n // 5 % 100).float(),
+            torch.where(n % 2 == 0, -0.0, 0.0), torch.where(n % 3 == 0, -0.0, torch.where(n % 3 == 1, 0.0, -1.0))]
     x = torch.stack(rows).to(dtype)
     for top in (1, 17, 32):
         _check(x, torch.full((len(rows),), V // 2, device="cuda"), top)

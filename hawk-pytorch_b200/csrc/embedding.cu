@@ -11,12 +11,13 @@
 //              8 B, against rows of kilobytes): it counts those of the blocks before it, which gives its place in the result
 //              without a word from them, and queues its own in shared memory in their order.  The queue's warps rank equal ids
 //              among their 32 (match.any) and take turns at the counters.
-//   2. windows sums of 16 consecutive places, only for windows inside the run of an id with more than 32 of them: the most
-//              frequent token of a text is 5 to 10 % of it, and one warp would walk its rows alone.
-//   3. rows    a warp per 8 table rows and 512 columns walks the places of its rows as one stream, three rows of dout ahead
-//              whichever table rows they belong to (most have no position or one: a loop per row would wait for each); zeros where
-//              there is nothing.  Long runs it passes over: the first blocks add them up from the windows' sums and ragged ends.
+//   2. windows sums of 8 consecutive places that lie in a run of more than 16 positions of one id (the most frequent token of a text is 5
+//              to 10 % of it, and one warp would walk its rows alone).
+//   3. rows    a warp per 8 table rows and 512 columns walks the places of its rows as one stream, three rows of dout ahead whichever
+//              table rows they belong to (most have no position or one: a loop per row would wait for each); zeros where there is
+//              nothing.  Long runs it passes over: the first blocks add them up from their windows' sums and ragged ends.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -31,6 +32,29 @@ template <>
 struct VecIO<__nv_bfloat16, 1> {
   static __device__ __forceinline__ void load(const __nv_bfloat16* p, float (&v)[1]) { v[0] = __bfloat162float(__ldg(p)); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, const float (&v)[1]) { *p = __float2bfloat16(v[0]); }
+};
+
+// VEC elements as they are stored
+template <typename T, int VEC>
+struct Raw {
+  static constexpr int B = VEC * sizeof(T);
+  using type = std::conditional_t<B == 16, uint4, std::conditional_t<B == 8, uint2, std::conditional_t<B == 4, uint32_t, uint16_t>>>;
+  static __device__ __forceinline__ type load(const T* p) { return __ldg(reinterpret_cast<const type*>(p)); }
+  static __device__ __forceinline__ void unpack(const type& r, float (&v)[VEC]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[j] = reinterpret_cast<const float*>(&r)[j];
+    } else if constexpr (VEC == 1) {
+      v[0] = __uint_as_float((uint32_t)r << 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 2) {
+        const float2 f = unpack_bf16x2(reinterpret_cast<const uint32_t*>(&r)[j / 2]);
+        v[j] = f.x;
+        v[j + 1] = f.y;
+      }
+    }
+  }
 };
 
 // ---- forward: 2^log_tpr threads to a row, four vectors of each in flight -----------------------------------
@@ -60,27 +84,28 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int64_t* __restric
 }
 
 // ---- backward 1: positions grouped by id ---------------------------------------------------------------------
-// Where the positions of id v come in the order of the groups: those of block v mod 2^log_blocks together, and there the ids whose
-// quotients lie slots / 8 apart next to one another, so that the 8 table rows of a warp are one that may be frequent and 7 rarer ones
-// (8 neighbouring quotients: the first warp had 8 rows of 60 positions each to add, 158 us where 60 were left to do).
+// Where the positions of id v come in the order of the groups: with those of its block, and there the ids whose quotients lie
+// slots / 8 apart next to one another, so that the 8 table rows of a warp are one that may be frequent and 7 rarer ones (8
+// neighbouring quotients: the first warp had 8 rows of 60 positions each to add, 158 us where 60 were left to do).  Low ids go to
+// all blocks alike (the frequent tokens of a vocabulary have them), and so do ids any power of two apart.
 constexpr int kRowGroup = 8;
 struct EmbedOrder {
   int log_blocks, slots;  // slots: ids of a block, a multiple of kRowGroup
   __host__ __device__ int64_t groups() const { return (int64_t)slots << log_blocks; }
+  __device__ int block(int64_t v) const { return (int)(v + (v >> log_blocks) * 37) & ((1 << log_blocks) - 1); }
   __device__ int slot(int64_t v) const {  // within its block
     const int x = (int)(v >> log_blocks), q = slots / kRowGroup;
     return x % q * kRowGroup + x / q;
   }
-  __device__ int64_t place(int64_t v) const { return (v & ((1 << log_blocks) - 1)) * slots + slot(v); }
-  __device__ int64_t id(int64_t place) const {  // the inverse
-    const int64_t block = place / slots, s = place % slots;
-    return (s % kRowGroup * (slots / kRowGroup) + s / kRowGroup) << log_blocks | block;
+  __device__ int64_t id(int64_t place) const {  // of the slot at place block * slots + slot
+    const int64_t b = place / slots, s = place % slots, x = s % kRowGroup * (slots / kRowGroup) + s / kRowGroup;
+    return x << log_blocks | ((b - x * 37) & ((1 << log_blocks) - 1));
   }
 };
 constexpr int kGroupThreads = 1024, kIdsPerThread = 8, kGroupStep = kGroupThreads * kIdsPerThread;
-constexpr int kQueue = kGroupStep;  // one step's ids always fit
+constexpr int kMinQueue = kGroupStep, kMaxQueue = 3 * kGroupStep;  // one step's ids always fit; 192 KB at most
 constexpr int kMaxSlots = 4096, kMinLogBlocks = 7;
-constexpr int kWindow = 16, kLong = 2 * kWindow;  // a run of more than kLong positions holds a whole window
+constexpr int kWindow = 8, kLong = 2 * kWindow;  // a run of more than kLong positions holds a whole window
 
 // exclusive sum over the block's threads; `all`: of all of them.  The shared words may be reused after the next barrier.
 __device__ __forceinline__ int block_scan(int v, int* warp_sums, int& all) {
@@ -121,12 +146,12 @@ struct StepIds {
     }
   }
   // which of them are this block's; `below` counts those of the blocks before it
-  __device__ __forceinline__ uint32_t mine(int64_t V, int64_t padding, int log_blocks, int block, int& below) const {
+  __device__ __forceinline__ uint32_t mine(int64_t V, int64_t padding, EmbedOrder order, int block, int& below) const {
     uint32_t m = 0;
 #pragma unroll
     for (int q = 0; q < kIdsPerThread; ++q) {
       if (id[q] < 0 || id[q] >= V || id[q] == padding) continue;
-      const int b = (int)id[q] & ((1 << log_blocks) - 1);
+      const int b = order.block(id[q]);
       below += b < block;
       if (b == block) m |= 1u << q;
     }
@@ -134,7 +159,7 @@ struct StepIds {
   }
 };
 
-// hands out the places of n <= kQueue queued (slot, position) pairs; the whole block
+// hands out the places of n queued (slot, position) pairs; the whole block
 __device__ __forceinline__ void place(const uint2* queue, int n, int* cursor, int* perm) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int k = 0; k < n; k += kGroupThreads) {
@@ -163,12 +188,15 @@ __device__ __forceinline__ void place(const uint2* queue, int n, int* cursor, in
 
 __global__ void __launch_bounds__(kGroupThreads) embed_group_kernel(const int64_t* __restrict__ ids, int64_t N, int64_t V, int64_t padding,
                                                                     EmbedOrder order, int* __restrict__ perm, int* __restrict__ start,
-                                                                    int* __restrict__ owner, int windows) {
-  extern __shared__ uint2 queue[];                       // [kQueue]
-  int* count = reinterpret_cast<int*>(queue + kQueue);   // [slots], the cursors later
+                                                                    int* __restrict__ owner, int4* __restrict__ runs, int windows,
+                                                                    int queue_size) {
+  extern __shared__ uint2 queue[];                           // [queue_size]
+  int* count = reinterpret_cast<int*>(queue + queue_size);   // [slots], the cursors later
   __shared__ int warp_sums[2][32];
-  const int tid = threadIdx.x, slots = order.slots, log_blocks = order.log_blocks;
+  __shared__ int nruns;
+  const int tid = threadIdx.x, slots = order.slots;
   for (int j = tid; j < slots; j += kGroupThreads) count[j] = 0;
+  if (tid == 0) nruns = 0;
   int below = 0, total = 0, all, step = 0;
   StepIds s, next;
   s.load(ids, tid * kIdsPerThread, N);
@@ -176,14 +204,14 @@ __global__ void __launch_bounds__(kGroupThreads) embed_group_kernel(const int64_
   for (int64_t base = 0; base < N; base += kGroupStep, step ^= 1) {  // the scans take turns with their shared words
     const int64_t i0 = base + tid * kIdsPerThread;
     if (base + kGroupStep < N) next.load(ids, i0 + kGroupStep, N);
-    const uint32_t mine = s.mine(V, padding, log_blocks, blockIdx.x, below);
+    const uint32_t mine = s.mine(V, padding, order, blockIdx.x, below);
     int at = total + block_scan(__popc(mine), warp_sums[step], all);
 #pragma unroll
     for (int q = 0; q < kIdsPerThread; ++q)
       if (mine >> q & 1) {
         const int j = order.slot(s.id[q]);
         atomicAdd(&count[j], 1);
-        if (at < kQueue) queue[at] = make_uint2((uint32_t)j, (uint32_t)(i0 + q));
+        if (at < queue_size) queue[at] = make_uint2((uint32_t)j, (uint32_t)(i0 + q));
         ++at;
       }
     total += all;
@@ -209,10 +237,13 @@ __global__ void __launch_bounds__(kGroupThreads) embed_group_kernel(const int64_
     const int j = tid * kPer + q;
     if (j < slots) count[j] = mystart[j] = at;
     at += c[q];
+    if (windows > 0 && c[q] > kLong)  // in any order
+      runs[(int64_t)blockIdx.x * (slots + 1) + 1 + atomicAdd(&nruns, 1)] = make_int4(at - c[q], at, (int)blockIdx.x * slots + j, 0);
   }
   const int behind = ahead + total;
-  if (blockIdx.x == gridDim.x - 1 && tid == 0) mystart[slots] = behind;
   __syncthreads();
+  if (windows > 0 && tid == 0) runs[(int64_t)blockIdx.x * (slots + 1)] = make_int4(nruns, 0, 0, 0);
+  if (blockIdx.x == gridDim.x - 1 && tid == 0) mystart[slots] = behind;
   // whose long run each window lies in (-1: none): the windows that start in this block's share, and those behind the last share
   const int w_end = blockIdx.x == gridDim.x - 1 ? windows : min(windows, (behind + kWindow - 1) / kWindow);
   for (int w = (ahead + kWindow - 1) / kWindow + tid; w < w_end; w += kGroupThreads) {
@@ -225,14 +256,14 @@ __global__ void __launch_bounds__(kGroupThreads) embed_group_kernel(const int64_
     owner[w] = end - count[lo] > kLong && (w + 1) * kWindow <= end ? (int)(blockIdx.x * slots + lo) : -1;
   }
   __syncthreads();
-  if (total <= kQueue) {
+  if (total <= queue_size) {
     place(queue, total, count, perm);
     return;
   }
   for (int64_t base = 0; base < N; base += kGroupStep, step ^= 1) {  // more than the queue holds: read the ids again
     const int64_t i0 = base + tid * kIdsPerThread;
     s.load(ids, i0, N);
-    const uint32_t mine = s.mine(V, padding, log_blocks, blockIdx.x, below);
+    const uint32_t mine = s.mine(V, padding, order, blockIdx.x, below);
     int to = block_scan(__popc(mine), warp_sums[step], all);
 #pragma unroll
     for (int q = 0; q < kIdsPerThread; ++q)
@@ -258,25 +289,29 @@ __global__ void __launch_bounds__(256) embed_window_kernel(const T* __restrict__
   const int lane = threadIdx.x & 31, win = (int)(unit / narrow), c0 = ((int)(unit % narrow) * 32 + lane) * VEC;
   if (owner[win] < 0) return;
   const int mine = perm[win * kWindow + lane % kWindow];
-  float v[kWindow][VEC], acc[VEC];
+  typename Raw<T, VEC>::type v[kWindow];
 #pragma unroll
   for (int r = 0; r < kWindow; ++r) {
     const int64_t p = __shfl_sync(0xffffffffu, mine, r);
-    if (c0 < H) VecIO<T, VEC>::load(dout + p * H + c0, v[r]);
+    if (c0 < H) v[r] = Raw<T, VEC>::load(dout + p * H + c0);
   }
+  float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
 #pragma unroll
-  for (int r = 0; r < kWindow; ++r)
+  for (int r = 0; r < kWindow; ++r) {
+    float x[VEC];
+    Raw<T, VEC>::unpack(v[r], x);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] += v[r][j];
+    for (int j = 0; j < VEC; ++j) acc[j] += x[j];
+  }
   if (c0 < H) VecIO<float, VEC>::store(partial + (int64_t)win * H + c0, acc);
 }
 
-// acc += n rows of `src`, the k-th of them row(k), one after the other; 32 values per lane in flight
+// acc += n rows of `src`, the k-th of them row(k), one after the other; 16 values per lane in flight, 2 rows at least
 template <typename T, int VEC, typename Row>
 __device__ __forceinline__ void add_rows(float (&acc)[VEC], const T* src, int H, int c0, int n, Row row) {
-  constexpr int D = VEC == 1 ? 16 : 32 / VEC;
+  constexpr int D = 16 / VEC;
 #pragma unroll 1
   for (int k = 0; k < n; k += D) {
     float v[D][VEC];
@@ -292,41 +327,74 @@ __device__ __forceinline__ void add_rows(float (&acc)[VEC], const T* src, int H,
   }
 }
 
-// the row of an id with a long run, by the units of its first window: 32 * VEC columns of the ragged ends, then of the windows' sums
+// The rows of the ids with long runs of one block of the order, 32 * VEC columns: a warp to a run, and all eight to a run of more than
+// kWarpWindows windows (each some of them, added up in their order).  `runs`: per block their number, then {first place, end, place of
+// the id} of each.
+constexpr int kWarpWindows = 16;
 template <typename T, int VEC>
-__device__ __forceinline__ void long_run(const T* dout, const int* perm, const int* start, const float* partial, const int* owner, T* dw,
-                                         EmbedOrder order, int H, float scale, int narrow, int64_t unit) {
-  const int win = (int)(unit / narrow), k = owner[win], c0 = ((int)(unit % narrow) * 32 + (threadIdx.x & 31)) * VEC;
-  if (k < 0 || c0 >= H) return;
-  const int s = start[k], e = start[k + 1], w1 = e / kWindow, head = win * kWindow - s, tail = e - w1 * kWindow;
-  if (head >= kWindow) return;
+__device__ __forceinline__ void add_runs(const T* dout, const int* perm, const float* partial, const int4* runs, T* dw, EmbedOrder order, int H,
+                                         float scale, int narrow) {
+  __shared__ __align__(16) float sums[8][32 * VEC];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x / narrow, c0 = (blockIdx.x % narrow * 32 + lane) * VEC;
+  const int4* list = runs + (int64_t)b * (order.slots + 1);
+  const int n = list[0].x;
   float acc[VEC];
+  const auto add_part = [&](int s, int e, int parts, int part) {  // of the windows, with the ragged ends in the first and last part
+    const int w0 = (s + kWindow - 1) / kWindow, w1 = e / kWindow, per = (w1 - w0 + parts - 1) / parts;
+    const int u0 = min(w0 + part * per, w1), u1 = min(u0 + per, w1);
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  add_rows<T, VEC>(acc, dout, H, c0, head + tail, [&](int i) { return perm[i < head ? s + i : w1 * kWindow + i - head]; });
-  add_rows<float, VEC>(acc, partial, H, c0, w1 - win, [&](int i) { return win + i; });
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    if (c0 >= H) return;
+    if (part == 0) add_rows<T, VEC>(acc, dout, H, c0, w0 * kWindow - s, [&](int r) { return perm[s + r]; });
+    add_rows<float, VEC>(acc, partial, H, c0, u1 - u0, [&](int w) { return u0 + w; });
+    if (part == parts - 1) add_rows<T, VEC>(acc, dout, H, c0, e - w1 * kWindow, [&](int r) { return perm[w1 * kWindow + r]; });
+  };
+  const auto write = [&](int place) {
+    if (c0 >= H) return;
 #pragma unroll
-  for (int j = 0; j < VEC; ++j) acc[j] *= scale;
-  VecIO<T, VEC>::store(dw + order.id(k) * H + c0, acc);
+    for (int j = 0; j < VEC; ++j) acc[j] *= scale;
+    VecIO<T, VEC>::store(dw + order.id(place) * H + c0, acc);
+  };
+  for (int base = 0; base < n; base += 32) {
+    int4 mine = base + lane < n ? list[1 + base + lane] : make_int4(0, 0, 0, 0);
+    const uint32_t big = __ballot_sync(0xffffffffu, mine.y - mine.x > kWarpWindows * kWindow);
+#pragma unroll 1
+    for (int i = 0; i < min(32, n - base); ++i) {
+      const int s = __shfl_sync(0xffffffffu, mine.x, i), e = __shfl_sync(0xffffffffu, mine.y, i), place = __shfl_sync(0xffffffffu, mine.z, i);
+      const bool all = big >> i & 1;
+      if (!all && i % 8 != warp) continue;
+      add_part(s, e, all ? 8 : 1, all ? warp : 0);
+      if (all) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) sums[warp][lane * VEC + j] = acc[j];
+        __syncthreads();
+        if (warp == 0)
+#pragma unroll
+          for (int w = 1; w < 8; ++w)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] += sums[w][lane * VEC + j];
+        __syncthreads();
+      }
+      if (!all || warp == 0) write(place);
+    }
+  }
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict__ dout, const int* perm, const int* start, const float* partial,
-                                                         const int* owner, T* __restrict__ dw, EmbedOrder order, int64_t V, int H,
-                                                         float scale, int chunks, int64_t units, int narrow, int64_t long_units) {
+__global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict__ dout, const int* perm, const int* start, const int4* runs,
+                                                            const float* partial, T* __restrict__ dw, EmbedOrder order, int64_t V, int H,
+                                                            float scale, int chunks, int64_t units, int narrow, int run_blocks) {
   constexpr int U = unit_vectors<T>(VEC);
   pdl_wait();
-  int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit < long_units) {  // long runs first: they take longest
-    long_run<T, VEC>(dout, perm, start, partial, owner, dw, order, H, scale, narrow, unit);
+  if ((int)blockIdx.x < run_blocks) {  // first: they take longest
+    add_runs<T, VEC>(dout, perm, partial, runs, dw, order, H, scale, narrow);
     return;
   }
-  unit -= long_units;
+  const int64_t unit = (int64_t)(blockIdx.x - run_blocks) * 8 + (threadIdx.x >> 5);
   if (unit >= units) return;
   const int lane = threadIdx.x & 31;
   const int64_t k0 = unit / chunks * kRowGroup;
   const int c0 = ((int)(unit % chunks) * 32 * U + lane) * VEC;
-  const int64_t id0 = order.id(k0), apart = (int64_t)(order.slots / kRowGroup) << order.log_blocks;
   const int st = start[k0 + min(lane, kRowGroup)];
   const int first = __shfl_sync(0xffffffffu, st, 0), last = __shfl_sync(0xffffffffu, st, kRowGroup);
   float acc[U][VEC];
@@ -337,7 +405,7 @@ __global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict_
       for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
   };
   const auto write = [&](int row) {
-    const int64_t v = id0 + row * apart;
+    const int64_t v = order.id(k0 + row);
     if (v >= V) return;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -349,23 +417,23 @@ __global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict_
       }
   };
   // the places of all rows as one stream, three rows of dout ahead; long runs are passed over
-  float v0[U][VEC], v1[U][VEC], v2[U][VEC];
+  typename Raw<T, VEC>::type v0[U], v1[U], v2[U];
   int pbase = first, places = first + lane < last ? perm[first + lane] : 0;  // 32 places, one per lane
   int i = first, ahead = first, bound = first, row = -1;  // v2, v1, v0 hold places ahead - 1, - 2, - 3
-  uint32_t runs = 0;                                      // rows that are long runs
+  uint32_t long_rows = 0;
   clear();
 #pragma unroll 1
   for (;;) {
 #pragma unroll 1
     while (i == bound) {  // the row ends here (and any empty ones behind it)
-      if (row >= 0 && !(runs >> row & 1)) {
+      if (row >= 0 && !(long_rows >> row & 1)) {
         write(row);
         clear();
       }
       if (++row == kRowGroup) break;
       bound = __shfl_sync(0xffffffffu, st, row + 1);
       if (bound - i > kLong) {
-        runs |= 1u << row;
+        long_rows |= 1u << row;
         i = ahead = bound;
       }
     }
@@ -373,12 +441,10 @@ __global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict_
 #pragma unroll 1
     do {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          v0[u][j] = v1[u][j];
-          v1[u][j] = v2[u][j];
-        }
+      for (int u = 0; u < U; ++u) {
+        v0[u] = v1[u];
+        v1[u] = v2[u];
+      }
       if (ahead < last) {
         if (ahead - pbase >= 32) {
           pbase = ahead;
@@ -387,14 +453,17 @@ __global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict_
         const T* p = dout + (int64_t)__shfl_sync(0xffffffffu, places, ahead - pbase) * H + c0;
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (c0 + u * 32 * VEC < H) VecIO<T, VEC>::load(p + u * 32 * VEC, v2[u]);
+          if (c0 + u * 32 * VEC < H) v2[u] = Raw<T, VEC>::load(p + u * 32 * VEC);
       }
       ++ahead;
     } while (ahead - 3 < i);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      float x[VEC];
+      Raw<T, VEC>::unpack(v0[u], x);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[u][j] += v0[u][j];
+      for (int j = 0; j < VEC; ++j) acc[u][j] += x[j];
+    }
     ++i;
   }
 }
@@ -403,7 +472,7 @@ __global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict_
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 struct EmbedWs {
-  size_t perm, start, partial, owner, total;
+  size_t perm, start, partial, owner, runs, total;
 };
 // as many blocks as nearly fill the GPU, more where a block's counters would not fit its shared memory
 static EmbedOrder embed_order(int64_t V) {
@@ -421,6 +490,8 @@ static EmbedWs embed_ws(int64_t N, int64_t V, int64_t H) {
   L.start = o;   o += up256((size_t)(embed_order(V).groups() + 1) * 4);
   L.partial = o; o += N > kLong ? up256((size_t)(N / kWindow) * H * 4) : 0;
   L.owner = o;   o += N > kLong ? up256((size_t)(N / kWindow) * 4) : 0;
+  const EmbedOrder order = embed_order(V);
+  L.runs = o;    o += N > kLong ? up256((size_t)(order.groups() + (1LL << order.log_blocks)) * sizeof(int4)) : 0;
   L.total = o;
   return L;
 }
@@ -449,19 +520,20 @@ static int embed_fwd(const int64_t* ids, const void* w, void* out, int64_t N, in
 }
 
 template <typename T, int VEC>
-static int embed_sums(const void* dout, void* dw, const int* perm, const int* start, float* partial, const int* owner, EmbedOrder order,
+static int embed_sums(const void* dout, void* dw, const int* perm, const int* start, float* partial, const int* owner, const int4* runs, EmbedOrder order,
                       int64_t N, int64_t V, int H, float scale, cudaStream_t st) {
   const int cols = 32 * VEC * unit_vectors<T>(VEC), chunks = (H + cols - 1) / cols, narrow = (H + 32 * VEC - 1) / (32 * VEC);
   const int64_t windows = N > kLong ? N / kWindow * narrow : 0, rows = order.groups() / kRowGroup * chunks;
-  HAWK_REQUIRE((rows + windows + 7) / 8 < (1LL << 31), HAWK_ERR_SHAPE);
+  const int64_t run_blocks = windows ? (int64_t)narrow << order.log_blocks : 0;
+  HAWK_REQUIRE((rows + 7) / 8 + run_blocks < (1LL << 31) && (windows + 7) / 8 < (1LL << 31), HAWK_ERR_SHAPE);
   const auto* g = static_cast<const T*>(dout);
   if (windows) {
     const int rc = launch_kernel(embed_window_kernel<T, VEC>, dim3((unsigned)((windows + 7) / 8)), dim3(256), 0, st, true, 1, g, perm, owner,
                                  partial, H, narrow, windows);
     if (rc != HAWK_OK) return rc;
   }
-  return launch_kernel(embed_rows_kernel<T, VEC>, dim3((unsigned)((rows + windows + 7) / 8)), dim3(256), 0, st, true, 1, g, perm, start,
-                       partial, owner, static_cast<T*>(dw), order, V, H, scale, chunks, rows, narrow, windows);
+  return launch_kernel(embed_rows_kernel<T, VEC>, dim3((unsigned)((rows + 7) / 8 + run_blocks)), dim3(256), 0, st, true, 1, g, perm, start, runs,
+                       partial, static_cast<T*>(dw), order, V, H, scale, chunks, rows, narrow, (int)run_blocks);
 }
 
 #define HAWK_BY_VEC(f, dtype, vec, ...)                                                                      \
@@ -504,15 +576,17 @@ extern "C" int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dw
   auto* owner = reinterpret_cast<int*>(ws + L.owner);
   const int windows = N > kLong ? (int)(N / kWindow) : 0;
   const EmbedOrder order = embed_order(V);
-  const size_t smem = kQueue * sizeof(uint2) + (size_t)order.slots * sizeof(int);
+  auto* runs = reinterpret_cast<int4*>(ws + L.runs);
+  const int queue = (int)std::min<int64_t>(kMaxQueue, std::max<int64_t>(kMinQueue, N));
+  const size_t smem = queue * sizeof(uint2) + (size_t)order.slots * sizeof(int);
   if (cudaFuncSetAttribute(embed_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
     (void)cudaGetLastError();
     return HAWK_ERR_LAUNCH;
   }
-  embed_group_kernel<<<1u << order.log_blocks, kGroupThreads, smem, st>>>(ids, N, V, padding_idx, order, perm, start, owner, windows);
+  embed_group_kernel<<<1u << order.log_blocks, kGroupThreads, smem, st>>>(ids, N, V, padding_idx, order, perm, start, owner, runs, windows, queue);
   const int rc = launch_status();
   if (rc != HAWK_OK) return rc;
   const int vec = common_vec((int)H, es, dout, dweight);
   return HAWK_BY_VEC(embed_sums, dtype, vec, dout, dweight, perm, start, reinterpret_cast<float*>(ws + L.partial),
-                     owner, order, N, V, (int)H, scale, st);
+                     owner, runs, order, N, V, (int)H, scale, st);
 }

@@ -1958,7 +1958,7 @@ def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, V: int, scale: float, p
         return torch.zeros(V, H, dtype=dout.dtype, device=dout.device)
     dw = torch.empty(V, H, dtype=dout.dtype, device=dout.device)
     ws = torch.empty(lib.hawk_embedding_bwd_workspace_bytes(N, V, H), dtype=torch.uint8, device=dout.device)
-    with _on(dout, "embedding_bwd", 3 if N > 32 else 2):
+    with _on(dout, "embedding_bwd", 3 if N > 16 else 2):
         _lib.check(lib.hawk_embedding_bwd(ids.data_ptr(), dout.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), N, V, H,
                                           padding_idx, scale, _dt(dout), _stream(dout)), "hawk_embedding_bwd")
     return dw

@@ -174,3 +174,10 @@ def test_module_and_model():
     sparse = M.Embedding(50, 24, sparse=True).cuda()
     sparse(ids).sum().backward()
     assert sparse.weight.grad.is_sparse
+
+
+@pytest.mark.parametrize("n,V", [(24576, 1), (24577, 1), (60000, 300), (200000, 40)])
+def test_runs_longer_than_a_queue(n, V):
+    """Blocks whose share is more than their queue holds, and runs of thousands of windows."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    _check(_zipf(n, V, g), V, 8, F32)

@@ -549,55 +549,64 @@ template <typename T>
 __global__ void __launch_bounds__(kLpBwdThreads) lp_bwd_kernel(LpBwdArgs a) {
   constexpr int N = RowVec<T>::N;
   const int64_t r = blockIdx.x / a.shares;
-  const int i0 = (int)(blockIdx.x % a.shares) * kLpBwdShare + threadIdx.x;
-  const int64_t token = a.tokens[r];
+  const int share = (int)(blockIdx.x % a.shares), i0 = share * kLpBwdShare + threadIdx.x;
   const Row<T> row(static_cast<const T*>(a.x) + r * a.ld, a.V);
+  const int w0 = row.whole(0) ? 0 : 1, w1 = row.whole(row.vectors - 1) ? row.vectors : row.vectors - 1;  // whole vectors
+  uint4 v[kLpBwdVectors];
+#pragma unroll
+  for (int q = 0; q < kLpBwdVectors; ++q) {  // requested before anything is known of the row
+    const int i = i0 + q * kLpBwdThreads;
+    if (i >= w0 && i < w1) v[q] = row.load_whole(i);
+  }
+  const int64_t token = a.tokens[r];
+  const float m = a.stats[2 * r], logs = a.stats[2 * r + 1], H = a.entropy[r], lp = a.logprob[r];
+  const float gl = a.g_lp ? a.g_lp[r] : 0.f, gh = a.g_ent ? a.g_ent[r] : 0.f;
   T* dx = static_cast<T*>(a.dx) + r * a.V;
   const bool same = ((reinterpret_cast<uintptr_t>(dx) ^ reinterpret_cast<uintptr_t>(row.p)) & 15) == 0;
-  uint4 v[kLpBwdVectors];
-  if (token >= 0)
-#pragma unroll
-    for (int q = 0; q < kLpBwdVectors; ++q)
-      if (i0 + q * kLpBwdThreads < row.vectors) v[q] = row.load(i0 + q * kLpBwdThreads);
-  const float m = a.stats[2 * r], logs = a.stats[2 * r + 1], H = a.entropy[r];
-  const float gl = a.g_lp ? a.g_lp[r] : 0.f, gh = a.g_ent ? a.g_ent[r] : 0.f;
+  const bool none = token < 0 || (m == -INFINITY && logs == -INFINITY);  // left out, or nothing but -infinity
+  const float nan = __int_as_float(0x7fc00000), scale = token >= a.V ? nan : -1.f;
+  const float k0 = fmaf(gh, H, gl), k1 = gh * kLn2;
+  // t = log2 p, floored where p is 0 (so that p t is): d = -p (gl + gh (log p + H))
+  const auto gradient = [&](float2 x) {
+    float2 t = mul2(add2(add2(x, f2(-m)), f2(-logs)), f2(kLog2e));
+    t = make_float2(max_nan(t.x, -200.f), max_nan(t.y, -200.f));
+    const float2 p = mul2(make_float2(ex2_approx(t.x), ex2_approx(t.y)), f2(scale)), g = mul2(p, fma2(t, f2(k1), f2(k0)));
+    return none ? f2(0.f) : g;
+  };
 #pragma unroll
   for (int q = 0; q < kLpBwdVectors; ++q) {
-    const int i = i0 + q * kLpBwdThreads;
-    if (i >= row.vectors) break;
-    float d[N];
-    if (token < 0 || (m == -INFINITY && logs == -INFINITY)) {  // left out, or nothing but -infinity
+    const int i = i0 + q * kLpBwdThreads, e = row.first(i);
+    if (i < w0 || i >= w1) continue;
+    float d[N], x[N];
+    RowVec<T>::unpack(v[q], x);
 #pragma unroll
-      for (int j = 0; j < N; ++j) d[j] = 0.f;
-    } else {
-      float x[N];
-      RowVec<T>::unpack(v[q], x);
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        float t;
-        const float p = lp_exp((x[j] - m) - logs, t);  // t: log2 p
-        d[j] = -p * fmaf(gh, fmaf(t, kLn2, H), gl);
-      }
-      const int64_t at = token - row.first(i);
-      if (at >= 0 && at < N) {
-        // 1 - p as -expm1(log p): the token is often all but certain
-        const float lp = a.logprob[r], own = fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp == -INFINITY ? 0.f : lp + H));
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (j == (int)at) d[j] = own;
-      }
-      if (token >= a.V)
-#pragma unroll
-        for (int j = 0; j < N; ++j) d[j] = __int_as_float(0x7fc00000);
+    for (int j = 0; j < N; j += 2) {
+      const float2 g = gradient(make_float2(x[j], x[j + 1]));
+      d[j] = g.x;
+      d[j + 1] = g.y;
     }
-    const int e = row.first(i);
-    if (same && row.whole(i)) {
+    if (same) {
       VecIO<T, N>::store(dx + e, d);
     } else {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (e + j >= 0 && e + j < a.V) dx[e + j] = from_float<T>(d[j]);
+      for (int j = 0; j < N; ++j) dx[e + j] = from_float<T>(d[j]);
     }
+  }
+  // elements of the row's cut vectors, by one warp of the first and last share
+  if (threadIdx.x < 32) {
+    for (int side = 0; side < 2; ++side) {
+      const int i = side == 0 ? 0 : row.vectors - 1;
+      if (row.whole(i) || i / kLpBwdShare != share || (side == 1 && i == 0)) continue;
+      const int e = row.first(i) + (int)threadIdx.x;
+      if ((int)threadIdx.x < N && e >= 0 && e < a.V) dx[e] = from_float<T>(gradient(f2(to_float(row.p[e]))).x);
+    }
+  }
+  // the token's own element anew, by the thread that wrote it: 1 - p as -expm1(log p), as the token is often all but certain
+  if (token >= 0 && token < a.V && !none) {
+    const int i = ((int)token + row.off) / N, in = i - share * kLpBwdShare;
+    const bool whole = i >= w0 && i < w1;
+    if (in >= 0 && in < kLpBwdShare && (int)threadIdx.x == (whole ? in % kLpBwdThreads : (int)token - row.first(i)))
+      dx[token] = from_float<T>(fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp == -INFINITY ? 0.f : lp + H)));
   }
 }
 

@@ -45,8 +45,9 @@ class GraphedDecoder:
         assert ids.shape[0] == self.batch_size
         for c in self.caches:
             c.current_cache_size = 0
-        self._latest = self._forward(ids)
-        return self._latest
+        logits = self._forward(ids)
+        self._latest = logits[:, -1:].clone()  # not a view, which would keep the whole prompt's logits
+        return logits
 
     def _capture(self):
         # warm up on a side stream (library handles, autotuning, allocator pools), keeping the cache

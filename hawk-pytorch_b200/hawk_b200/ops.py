@@ -852,7 +852,10 @@ def _status_word(device: torch.device) -> torch.Tensor:
     t = _ce_status.get(device.index)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=device)
-        _ce_status[device.index] = t
+        # While a graph is being captured the zeros are written by its replays, and the word lives in its memory: it serves this
+        # call alone (whose results show a failure by themselves), and the next eager call makes the shared one.
+        if not torch.cuda.is_current_stream_capturing():
+            _ce_status[device.index] = t
     return t
 
 

@@ -4,6 +4,7 @@ import math
 
 import pytest
 import torch
+import torch.utils._python_dispatch
 
 from conftest import rel_l2
 
@@ -150,12 +151,16 @@ def test_a_cached_model_refuses_whole_sequences():
 
 
 def test_through_the_dispatcher():
-    """The same calls where torch has to see the operators: under a mode and a profiler, and as torch.library's checks want them."""
+    """The same calls where torch has to see the operators: under modes, and as torch.library's checks want them."""
     import hawk_b200 as h
     from hawk_b200 import ops
 
     class Passes(torch.overrides.TorchFunctionMode):
         def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Dispatches(torch.utils._python_dispatch.TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
             return func(*args, **(kwargs or {}))
     g = torch.Generator(device="cuda").manual_seed(0)
     w = torch.randn(50, 64, generator=g, device="cuda").bfloat16().requires_grad_()
@@ -168,7 +173,7 @@ def test_through_the_dispatcher():
         grads = torch.autograd.grad([o.float().sum() for o in out if o.requires_grad], [w, a, x])
         return [*out, *grads]
     direct = everything()
-    for context in (Passes, torch.profiler.profile):
+    for context in (Passes, Dispatches):
         with context():
             seen = everything()
         assert all(torch.equal(p, q) for p, q in zip(direct, seen))
@@ -176,3 +181,79 @@ def test_through_the_dispatcher():
     torch.library.opcheck(ops.embedding_fwd, (ids.clamp(min=0), w, 2.0, 3), test_utils=tests)
     torch.library.opcheck(ops.token_logprobs_fwd, (x, ids, 4), test_utils=tests)
     torch.library.opcheck(ops.linear_logprobs_fwd, (w.detach(), a.detach(), ids, False), test_utils=tests[:1] + tests[2:3])
+
+
+def test_saved_bytes_are_what_the_fake_says():
+    from hawk_b200 import ops
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    for wdt, adt, V, N, H in [(torch.float32, torch.float32, 300, 5, 64), (torch.bfloat16, torch.bfloat16, 129, 70, 8),
+                              (torch.bfloat16, torch.float32, 1000, 33, 24)]:
+        for grad in (False, True):
+            args = (torch.zeros(V, H, dtype=wdt, device="cuda"), torch.zeros(N, H, dtype=adt, device="cuda"),
+                    torch.zeros(N, dtype=torch.int64, device="cuda"))
+            real = ops.linear_logprobs_fwd(*args, grad)
+            with FakeTensorMode() as mode:
+                fake = ops.linear_logprobs_fwd(*(mode.from_tensor(a) for a in args), grad)
+            assert [t.shape for t in real] == [t.shape for t in fake] and [t.dtype for t in real] == [t.dtype for t in fake]
+
+
+def test_a_first_call_inside_a_capture():
+    """The status word of the tensor-core kernels made while capturing belongs to the graph: eager calls before its first replay
+    must not read it."""
+    from hawk_b200 import linear_logprobs, ops
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w, a = (torch.randn(200, 64, generator=g, device="cuda").bfloat16() for _ in range(2))
+    t = torch.randint(0, 200, (200,), generator=g, device="cuda")
+    want = linear_logprobs(w, a, t)
+    kept = dict(ops._ce_status)
+    torch.cuda.synchronize()
+    ops._ce_status.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = linear_logprobs(w, a, t)
+        assert not ops._ce_status
+        assert all(torch.equal(x, y) for x, y in zip(linear_logprobs(w, a, t), want))
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+        ops.check_device_status()
+    finally:
+        ops._ce_status.update(kept)
+
+
+def test_prompt_logits_are_not_kept():
+    from hawk_b200.generate import GraphedDecoder
+    m = _model(5, use_cache=True).bfloat16()
+    dec = GraphedDecoder(m, 2, autocast=False, use_graph=False)
+    logits = dec.prefill(torch.randint(1, 96, (2, 50), device="cuda"))
+    assert dec._latest.untyped_storage().nbytes() == logits[:, -1].numel() * logits.element_size()
+    assert torch.equal(dec._latest[:, 0], logits[:, -1])
+
+
+def test_two_calls_at_once_on_two_streams():
+    """Nothing is shared between calls but the status word."""
+    from hawk_b200 import embedding, grad_norm, linear_logprobs, ops, token_logprobs
+    g = torch.Generator(device="cuda").manual_seed(3)
+    sets = []
+    for k in range(2):
+        w = torch.randn(3000, 128, generator=g, device="cuda").bfloat16()
+        a = torch.randn(700, 128, generator=g, device="cuda").bfloat16()
+        t = torch.randint(0, 3000, (700,), generator=g, device="cuda")
+        sets.append((w, a, t, torch.randn(700, 3000, generator=g, device="cuda")))
+
+    def run(w, a, t, x):
+        lp, H, saved = ops.linear_logprobs_fwd(w, a, t, True)
+        return [lp, H, *ops.linear_logprobs_bwd(w, a, t, saved, lp, H, lp, H, True, True), *token_logprobs(x, t, 7), embedding(t, w, 2.0),
+                ops.embedding_bwd(t, a, 3000, 1.0, -1), grad_norm([w, a, x])]
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(run(*sets[k]))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for out in got[k]:
+            assert all(torch.equal(x, y) for x, y in zip(out, want[k]))

@@ -69,16 +69,18 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const int64_t* __restric
   const T* src = w + (known ? id : 0) * H;
   T* dst = out + row * H;
   for (int c0 = (threadIdx.x & (tpr - 1)) * VEC; c0 < H; c0 += 4 * tpr * VEC) {
-    float v[4][VEC];
+    typename Raw<T, VEC>::type r[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (c0 + u * tpr * VEC < H) VecIO<T, VEC>::load(src + c0 + u * tpr * VEC, v[u]);
+      if (c0 + u * tpr * VEC < H) r[u] = Raw<T, VEC>::load(src + c0 + u * tpr * VEC);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (c0 + u * tpr * VEC < H) {
+        float v[VEC];
+        Raw<T, VEC>::unpack(r[u], v);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[u][j] = known ? v[u][j] * scale : __int_as_float(0x7fc00000);
-        VecIO<T, VEC>::store(dst + c0 + u * tpr * VEC, v[u]);
+        for (int j = 0; j < VEC; ++j) v[j] = known ? v[j] * scale : __int_as_float(0x7fc00000);
+        VecIO<T, VEC>::store(dst + c0 + u * tpr * VEC, v);
       }
   }
 }

@@ -5,13 +5,18 @@
     python -m hawk_b200.microbench gates     [--B 8 --T 4096 --D 2048 --bw 128]       # both gate projections
     python -m hawk_b200.microbench conv1d    [--B 8 --T 4096 --D 2048 --dtype bf16]
     python -m hawk_b200.microbench linear_ce [--N 32760 --H 2048 --V 32000]
+    python -m hawk_b200.microbench linear_logprobs [--N 32760 --H 2048 --V 32000]     # log probability and entropy, both ways
+    python -m hawk_b200.microbench token_logprobs [--N 256 --V 32000 --top 20 --dtype bf16]   # the same from logits, both ways
+    python -m hawk_b200.microbench embedding [--N 32768 --H 2048 --V 32000 --dtype f32]   # tokens as frequent as in text
+    python -m hawk_b200.microbench grad_norm [--layers 24]   # over the 1.35 B model's gradients
     python -m hawk_b200.microbench glue      [--N 32768 --H 2048 --J 6144]   # gelu(a)*b and add+RMSNorm, both ways
     python -m hawk_b200.microbench decode    [--B 256 --D 2048 --layers 24]
     python -m hawk_b200.microbench decode_model [--B 256]   # one cached token of the 1.35 B model, eager vs CUDA graph
 
 Prints one JSON line per kernel with the achieved rate against its algorithmic work:
 scan 8 (forward) / 16 (backward) bytes per element in bf16 (12 / 20 with the fused gelu(y)*h epilogue), gate
-projections 6 / 14, conv1d 4 / 6, linear_ce 6*N*H*V flop,
+projections 6 / 14, conv1d 4 / 6, linear_ce and linear_logprobs 6*N*H*V flop (2 forward), token_logprobs one read of
+the logits (and one write backward), embedding N rows written and the rows named read (backward N rows read, V written),
 decode 8*B*D*elem bytes per step; glue: the tensors each kernel must read and write once (gelu(a)*b:
 3 / 5 bf16 tensors of N x J; add+RMSNorm with an fp32 residual stream and bf16 branch: 12 / 16 bytes per
 element).  Inputs are seeded normal draws; Lambda sits on the reference's
@@ -58,7 +63,9 @@ def _emit(name, ms, work, unit, **extra):
 
 def main(argv=None):
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=["scan", "scan_gelu", "gates", "conv1d", "linear_ce", "glue", "decode", "decode_model"])
+    ap.add_argument("op", choices=["scan", "scan_gelu", "gates", "conv1d", "linear_ce", "linear_logprobs", "token_logprobs", "embedding",
+                                   "grad_norm", "glue", "decode", "decode_model"])
+    ap.add_argument("--top", type=int, default=20)
     ap.add_argument("--bw", type=int, default=128)
     ap.add_argument("--J", type=int, default=6144)
     ap.add_argument("--B", type=int, default=None)
@@ -171,6 +178,53 @@ def main(argv=None):
         t = _time(lambda: torch.autograd.grad(ops.fused_cross_entropy(w, act, lab), (w, act)), max(3, a.iters // 4), 2, flush)
         ops.check_device_status()
         _emit("linear_ce", t, 6 * a.N * a.H * a.V, "TFLOP/s", N=a.N, H=a.H, V=a.V)
+    elif a.op == "linear_logprobs":
+        w = (torch.randn(a.V, a.H, generator=g, device=dev) / math.sqrt(a.H)).bfloat16()
+        act = torch.randn(a.N, a.H, generator=g, device=dev).bfloat16()
+        tok = torch.randint(0, a.V, (a.N,), generator=g, device=dev)
+        up = torch.randn(a.N, generator=g, device=dev) / a.N
+        lp, ent, saved = ops.linear_logprobs_fwd(w, act, tok, True)
+        few = max(3, a.iters // 4)
+        size = {"N": a.N, "H": a.H, "V": a.V}
+        tf = _time(lambda: ops.linear_logprobs_fwd(w, act, tok, False), few, 2, flush)
+        tk = _time(lambda: ops.linear_logprobs_fwd(w, act, tok, True), few, 2, flush)
+        tb = _time(lambda: ops.linear_logprobs_bwd(w, act, tok, saved, lp, ent, up, up, True, True), few, 2, flush)
+        ops.check_device_status()
+        _emit("linear_logprobs_score", tf, 2 * a.N * a.H * a.V, "TFLOP/s", **size)
+        _emit("linear_logprobs_fwd", tk, 2 * a.N * a.H * a.V, "TFLOP/s", **size)
+        _emit("linear_logprobs_bwd", tb, 4 * a.N * a.H * a.V, "TFLOP/s", **size)
+    elif a.op == "token_logprobs":
+        N = 256 if a.N == 8 * 4095 else a.N
+        x = (2.5 * torch.randn(N, a.V, generator=g, device=dev)).to(dt)
+        tok = torch.randint(0, a.V, (N,), generator=g, device=dev)
+        up = torch.randn(N, generator=g, device=dev)
+        lp, ent, _, _, stats = ops.token_logprobs_fwd(x, tok, 0)
+        size = {"N": N, "V": a.V, "dtype": a.dtype}
+        for top in sorted({0, a.top}):
+            t = _time(lambda: ops.token_logprobs_fwd(x, tok, top), a.iters, a.warmup, flush)
+            _emit("token_logprobs_fwd", t, es * N * a.V, "GB/s", top=top, **size)
+        t = _time(lambda: ops.token_logprobs_bwd(x, tok, stats, lp, ent, up, up), a.iters, a.warmup, flush)
+        _emit("token_logprobs_bwd", t, 2 * es * N * a.V, "GB/s", **size)
+    elif a.op == "embedding":
+        N = 8 * 4096 if a.N == 8 * 4095 else a.N
+        ids = (float(a.V) ** torch.rand(N, generator=g, device=dev, dtype=torch.float64)).long().sub_(1).clamp_(0, a.V - 1)
+        w = torch.randn(a.V, a.H, generator=g, device=dev).to(dt)
+        go = torch.randn(N, a.H, generator=g, device=dev).to(dt)
+        size = {"N": N, "V": a.V, "H": a.H, "dtype": a.dtype}
+        tf = _time(lambda: ops.embedding_fwd(ids, w, 2.0, -1), a.iters, a.warmup, flush)
+        tb = _time(lambda: ops.embedding_bwd(ids, go, a.V, 2.0, -1), a.iters, a.warmup, flush)
+        _emit("embedding_fwd", tf, (N + ids.unique().numel()) * a.H * es, "GB/s", **size)
+        _emit("embedding_bwd", tb, (N + a.V) * a.H * es, "GB/s", **size)
+    elif a.op == "grad_norm":
+        from .model import HawkModel, hawk_1b_config
+        cfg = hawk_1b_config()
+        cfg.num_hidden_layers = a.layers
+        with torch.device("meta"):
+            shapes = [p.shape for p in HawkModel(cfg).parameters()]
+        grads = [torch.randn(s, generator=g, device=dev).to(dt) for s in shapes]
+        n = sum(t.numel() for t in grads)
+        _emit("grad_norm", _time(lambda: ops.grad_norm(grads), a.iters, a.warmup, flush), es * n, "GB/s", tensors=len(grads), elements=n,
+              dtype=a.dtype)
     elif a.op == "decode_model":
         from .generate import GraphedDecoder
         from .model import HawkModel, hawk_1b_config

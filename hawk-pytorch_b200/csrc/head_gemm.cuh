@@ -301,6 +301,11 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       int mt, nt;
       tile_coords(tile % tiles, m_tiles, n_tiles, mt, nt);
       const int acc = NACC == 2 ? (tcount & 1) : 0;
+      long long score_label = -1;  // requested before the wait: it is an L2 access away
+      if (MODE == EPI_SCORE || MODE == EPI_SCORE_KEEP) {
+        const int r = mt * BM + (int)rank * 128 + quarter * 32 + lane;
+        if (r < ep.M) score_label = __ldg(ep.labels + r);
+      }
       if (!mbar_wait_warp(&tfull_bar[acc], NACC == 2 ? ((tcount >> 1) & 1) : (tcount & 1), abortp)) break;  // lane 0 waits: the warp cannot diverge
       fence_after();
       const int col0 = nt * BN + half * EPI_COLS;
@@ -330,12 +335,20 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           }
         }
         const float m = fmaxf(m0, m1);
-        const long long label = row_ok ? ep.labels[row] : -1;
+        const long long label = score_label;
         float2 s = f2(0.f), sx = f2(0.f);
 #pragma unroll
         for (int c = 0; c < EPI_COLS / 32; ++c) {
           tmem_ld_wait();
-          if (c + 1 < EPI_COLS / 32) tmem_ld32_async(taddr0 + (c + 1) * 32, v[(c + 1) & 1]);
+          if (c + 1 < EPI_COLS / 32) {
+            tmem_ld32_async(taddr0 + (c + 1) * 32, v[(c + 1) & 1]);
+          } else {
+            // The accumulator is read: hand it back now.  The arrival is a release, which behind this tile's stores would wait for
+            // their way to L2 and back.
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_remote(map_to_rank(&tempty_bar[acc], 0));
+          }
           const int cbase = col0 + c * 32;
           uint32_t packed[16];
           float* correct = ep.correct + (row_ok ? row : 0);
@@ -418,9 +431,11 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
       }
       }  // halves
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_remote(map_to_rank(&tempty_bar[acc], 0));
+      if (MODE != EPI_SCORE && MODE != EPI_SCORE_KEEP) {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(map_to_rank(&tempty_bar[acc], 0));
+      }
     }
     if (lane == 0) bulk_wait_all();
   }

@@ -50,7 +50,7 @@ struct EpiParams {
   float2* stats;             // [column groups of 128, M] (max, sum exp)
   float* correct;            // [M] logit at the label
   const long long* labels;   // [M]
-  // EPI_SCORE, EPI_SCORE_KEEP (which also stores e^(x - max) in bf16): `correct` and `labels` as above, and
+  // EPI_SCORE, EPI_SCORE_KEEP (which also stores e^(x - max) in fp16): `correct` and `labels` as above, and
   float4* score;             // [M, column groups of 128] (max, sum exp, sum exp (x - max) log2 e, unused)
   int groups;                // column groups
   // EPI_OUT
@@ -115,7 +115,7 @@ __device__ __forceinline__ void softmax_chunk(const uint32_t (&v)[32], int cbase
 }
 
 // One 32-column chunk of unrounded logits of one row, whose group's maximum m is known: the sums of e = e^(x - m) and of
-// e (x - m) log2 e (for the entropy), the label's logit, and with KEEP e itself in bf16.
+// e (x - m) log2 e (for the entropy), the label's logit, and with KEEP e itself in fp16 (at most 1, so nothing overflows).
 template <bool FULL, bool KEEP>
 __device__ __forceinline__ void score_chunk(const uint32_t (&v)[32], float m, int cbase, int Nc, long long label, float* correct,
                                             uint32_t (&packed)[16], float2& s, float2& sx) {
@@ -130,7 +130,7 @@ __device__ __forceinline__ void score_chunk(const uint32_t (&v)[32], float m, in
     const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
     s = add2(s, e);
     sx = fma2(e, t, sx);
-    if (KEEP) packed[j] = pack_bf16x2(e.x, e.y);
+    if (KEEP) packed[j] = pack_f16x2(e.x, e.y);
   }
   if (label >= cbase && label < cbase + 32 && label < Nc) {
     const int at = (int)(label - cbase);

@@ -2,9 +2,9 @@
 // are never rounded and never in memory:
 //   1. GEMM (head_gemm.cuh) whose epilogue reduces every row's 128 columns, from the fp32 accumulators, to their maximum m_g,
 //      the sum of e = e^(x - m_g) and the sum of e (x - m_g) log2 e; the token's logit is picked out on the way.  Where a
-//      gradient is wanted it stores e, in bf16: at most 1, so its rounding is 2^-9 of a probability whatever the logits' size
-//      (a bf16 logit of 20 is off by 0.06, 6 % of its probability), and exactly 1 at each group's maximum, so that the
-//      probability of a token that all but certain is as exact as the sums.
+//      gradient is wanted it stores e, in fp16: at most 1, so its rounding is 2^-12 of a probability (2^-25 of the group's largest
+//      below 2^-14 of it) whatever the logits' size (a bf16 logit of 20 is off by 0.06, 6 % of its probability), and exactly 1 at
+//      each group's maximum, so that the probability of a token that is all but certain is as exact as the sums.
 //   2. reduce  a warp per row over its groups: m, log s, log probability and entropy.  The token's own logit is formed once more,
 //      as a plain fp32 dot product: the tensor core truncates its running sum at every step of 16 products, which leaves a large
 //      logit a little too small (2e-5 of 16 after 2048 products), and a log probability near 0 would be nothing but that.  The
@@ -80,7 +80,7 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
 constexpr int kDxThreads = 512;
 // d x of one row per block, 8 columns (16 bytes of e, of one group) per thread and step
 __global__ void __launch_bounds__(kDxThreads)
-score_dx_kernel(const __nv_bfloat16* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
+score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
                 const float* __restrict__ logprob, const float* __restrict__ entropy, const int64_t* __restrict__ tokens,
                 const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, long long ld, int V,
                 int groups) {
@@ -92,7 +92,7 @@ score_dx_kernel(const __nv_bfloat16* __restrict__ e, const float4* __restrict__ 
     for (int i = threadIdx.x; i < nvec; i += kDxThreads) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
-  const __nv_bfloat16* in = e + row * ld;
+  const __half* in = e + row * ld;
   const float4* g = score + row * groups;
   const float2 st = stats[row];
   const float lp = logprob[row], H = entropy[row], gl = g_lp ? g_lp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
@@ -106,7 +106,7 @@ score_dx_kernel(const __nv_bfloat16* __restrict__ e, const float4* __restrict__ 
     float d[8];
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const float2 ev = unpack_bf16x2(w[q]);
+      const float2 ev = unpack_f16x2(w[q]);
       float c0 = gl, c1 = gl;
       if (gh != 0.f) {  // the same for all of the row
         c0 = fmaf(gh, fmaf(fmaxf(__log2f(ev.x), -200.f), 0.6931471805599453f, off) + H, gl);  // e = 0: a finite factor
@@ -272,7 +272,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const auto* ab = static_cast<const __nv_bfloat16*>(a_dtype == HAWK_F32 ? static_cast<const void*>(sv + S.ab) : act);
   auto* dx = reinterpret_cast<__nv_bfloat16*>(sc + L.dx);
   auto* part = reinterpret_cast<float*>(sc + L.partial);
-  score_dx_kernel<<<(unsigned)N, kDxThreads, 0, st>>>(reinterpret_cast<const __nv_bfloat16*>(sv + S.e),
+  score_dx_kernel<<<(unsigned)N, kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
                                                       reinterpret_cast<const float4*>(sv + S.score),
                                                       reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, tokens, g_logprob,
                                                       g_entropy, dx, S.ldV, (int)V, S.groups);

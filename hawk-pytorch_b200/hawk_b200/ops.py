@@ -1919,7 +1919,7 @@ def linear_logprobs(weight, act, tokens):
     """(logprob, entropy) of `tokens` [..] under the distributions softmax(act @ weight.T): weight [V,H], act [..,H] (fp32 or bf16, H
     a multiple of 8), both results fp32 of tokens' shape and differentiable in weight and act.  What fused_cross_entropy is to the
     mean loss: bf16 tensor-core products (operands in fp32 are rounded, as there), but the logits stay unrounded fp32 sums and are
-    never in memory; a forward that waits for its backward holds N * V bf16 values.  Negative tokens and those >= V as in
+    never in memory; a forward that waits for its backward holds N * V 16-bit values.  Negative tokens and those >= V as in
     token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold."""
     if weight.dim() != 2 or act.dim() < 1 or act.shape[-1] != weight.shape[1]:
         raise ValueError(f"hawk_b200: activations of shape {tuple(act.shape)} with a weight of shape {tuple(weight.shape)}")

@@ -3,9 +3,10 @@ bf16 operands.
 
 Tolerances.  A logit is an fp32 sum of H exact products: off by less than H 2^-24 sum |a w| (measured far less: pairwise inside the
 tensor core); with |a||w| <= 8 sqrt(H) here and errors that do not conspire, 2^-20 of the logits' spread; log s adds 8e-6 as in
-the logits' own test: 3e-5 absolute in a log probability, 1e-4 in the entropy.  Gradients: d x is e rounded to bf16 (2^-9) times
-factors right to 1e-4, rounded to bf16 (2^-9): 2^-8 per element and, over sums of many, 2^-8 norm-wise; the result rounds once more
-(2^-9 in bf16): 6e-3 norm-wise."""
+the logits' own test: 3e-5 absolute in a log probability, 1e-4 in the entropy.  Gradients: d x is e rounded to fp16 (2^-12, or
+2^-25 of its group's largest) times factors right to 1e-4, rounded to bf16 (2^-8 half a step of eps 2^-7): 2^-8 + 4e-4 per element
+and, over sums of many, norm-wise; the result rounds once more (2^-8 in bf16).  Independent roundings of at most 2^-8 relative have
+a root mean square of 2^-8 / sqrt(3) or less: sqrt(2) of that, 3.2e-3; 6e-3 leaves room for few terms."""
 import math
 
 import pytest

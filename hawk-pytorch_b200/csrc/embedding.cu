@@ -585,7 +585,9 @@ extern "C" int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dw
   auto* runs = reinterpret_cast<int4*>(ws + L.runs);
   const int queue = (int)std::min<int64_t>(kMaxQueue, std::max<int64_t>(kMinQueue, N));
   const size_t smem = queue * sizeof(uint2) + (size_t)order.slots * sizeof(int);
-  if (cudaFuncSetAttribute(embed_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+  // always the most that any call takes: calls of two threads share this setting
+  constexpr int kMostSmem = kMaxQueue * (int)sizeof(uint2) + kMaxSlots * (int)sizeof(int);
+  if (cudaFuncSetAttribute(embed_group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostSmem) != cudaSuccess) {
     (void)cudaGetLastError();
     return HAWK_ERR_LAUNCH;
   }

@@ -181,3 +181,20 @@ def test_runs_longer_than_a_queue(n, V):
     """Blocks whose share is more than their queue holds, and runs of thousands of windows."""
     g = torch.Generator(device="cuda").manual_seed(n)
     _check(_zipf(n, V, g), V, 8, F32)
+
+
+def test_backward_from_two_threads():
+    """Calls whose blocks hold shared memory of different sizes: the kernel's limit belongs to the process."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from hawk_b200 import ops
+
+    def work(n, V):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            ids, go = torch.arange(n, device="cuda") % V, torch.ones(n, 8, device="cuda")
+            for _ in range(300):
+                dw = ops.embedding_bwd(ids, go, V, 1.0, -1)
+            return bool((dw == (n // V)).all())
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(work, (30000, 64), (500, 64)))

@@ -196,3 +196,15 @@ def test_trainer_clips():
     st = tr.opt.state[first]
     coef = min(1.0, 0.25 / (_norm64(grads) + 1e-6))
     assert rel_l2(st["exp_avg"], 0.1 * coef * grads[0].double()) <= 1e-6
+
+
+def test_a_step_without_gradients_has_no_norm():
+    from hawk_b200 import train
+    p = torch.nn.Parameter(torch.ones(100, device="cuda"))
+    opt = train.FusedAdamW([p], max_grad_norm=1.0)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert float(opt.grad_norm) == 10.0
+    p.grad = None
+    opt.step()
+    assert opt.grad_norm is None

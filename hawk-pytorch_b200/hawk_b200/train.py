@@ -48,10 +48,10 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     with torch.no_grad():
         table, device, keep = ops._norm_table(grads)
         both = ops._grad_norm(table, device, float(max_norm))
+        ops.scale_in_place([g for g in grads if g.is_contiguous()], both[1])  # first: it refuses gradients that share memory
         strided = [g for g in grads if not g.is_contiguous()]
-        if strided:  # neither copied nor listed twice: torch's own product, which knows strides
+        if strided:  # torch's own product, which knows strides
             torch._foreach_mul_(strided, both[1])
-        ops.scale_in_place([g for g in grads if g.is_contiguous()], both[1])
     return both[0]
 
 

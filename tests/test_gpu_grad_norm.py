@@ -208,3 +208,13 @@ def test_a_step_without_gradients_has_no_norm():
     p.grad = None
     opt.step()
     assert opt.grad_norm is None
+
+
+def test_a_refused_clip_changes_nothing():
+    from hawk_b200 import train
+    ps = [torch.nn.Parameter(torch.zeros(n, n, device="cuda")) for n in (8, 8, 6)]
+    ps[0].grad = ps[1].grad = torch.ones(8, 8, device="cuda")  # one tensor as the gradient of two parameters
+    ps[2].grad = torch.ones(6, 12, device="cuda")[:, ::2]
+    with pytest.raises(ValueError, match="share memory"):
+        train.clip_grad_norm_(ps, 0.5)
+    assert all(bool((p.grad == 1).all()) for p in ps)

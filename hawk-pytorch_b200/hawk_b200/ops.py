@@ -2059,7 +2059,9 @@ def _grad_norm(table, device, max_norm: float) -> torch.Tensor:
     if not max_norm >= 0:
         raise ValueError(f"hawk_b200: max_norm {max_norm} (a norm is not negative)")
     if not table:
-        return torch.tensor([0.0, min(1.0, max_norm / 1e-6)], device=device)
+        out = torch.zeros(2, device=device)
+        out[1] = min(1.0, max_norm / 1e-6)  # a fill, not a copy from the host, which would wait and cannot be captured
+        return out
     lib = _lib.load()
     count = len(table) // 3
     out = torch.empty(2, dtype=torch.float32, device=device)

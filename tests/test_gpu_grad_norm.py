@@ -218,3 +218,13 @@ def test_a_refused_clip_changes_nothing():
     with pytest.raises(ValueError, match="share memory"):
         train.clip_grad_norm_(ps, 0.5)
     assert all(bool((p.grad == 1).all()) for p in ps)
+
+
+def test_norm_of_nothing_can_be_captured():
+    from hawk_b200 import grad_norm
+    empty = [torch.empty(0, device="cuda"), torch.empty(3, 0, device="cuda")]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = grad_norm(empty)
+    graph.replay()
+    assert norm.is_cuda and float(norm) == 0.0 and float(grad_norm([])) == 0.0

@@ -2060,7 +2060,7 @@ def _grad_norm(table, device, max_norm: float) -> torch.Tensor:
         raise ValueError(f"hawk_b200: max_norm {max_norm} (a norm is not negative)")
     if not table:
         out = torch.zeros(2, device=device)
-        out[1] = min(1.0, max_norm / 1e-6)  # a fill, not a copy from the host, which would wait and cannot be captured
+        out[1:].fill_(min(1.0, max_norm / 1e-6))  # not a copy from the host, which would wait and cannot be captured
         return out
     lib = _lib.load()
     count = len(table) // 3

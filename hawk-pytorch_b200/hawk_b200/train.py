@@ -62,8 +62,8 @@ class FusedAdamW(torch.optim.Optimizer):
     forward casts nothing.  State keys follow torch.optim.AdamW (`step`, `exp_avg`, `exp_avg_sq`).
 
     `max_grad_norm`: every step takes the gradients of all groups times min(1, max_grad_norm / (norm + 1e-6)), where norm is
-    their global 2-norm before (`grad_norm` after the step: a scalar on the device, None where no parameter had a gradient).  `p.grad` itself is left as it is: the factor
-    is applied as the update reads it."""
+    their global 2-norm before (`grad_norm` after the step: a scalar on the device, None where no parameter had a
+    gradient).  `p.grad` itself is left as it is: the factor is applied as the update reads it."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, shadow_modules=(),
                  max_grad_norm: Optional[float] = None):

@@ -4,7 +4,7 @@
 // one-launch-per-tensor norms of a 315-tensor model are mostly launches); its blocks walk over the 32 KB chunks of all
 // tensors and leave one double each, which a second launch of one block adds up in a fixed order: the result does not
 // depend on timing.  The clip itself rides on the optimiser's read of the gradients (hawk_adamw_multi_scaled) or is a pass
-// of its own (hawk_scale_multi) that touches nothing where coef is 1.  A clipped AdamW step of 185 M parameters: norm 0.12 ms,
+// of its own (hawk_scale_multi) that touches nothing where coef is 1.  A clipped AdamW step of 182 M parameters: norm 0.12 ms,
 // update 0.75 ms.
 //
 // Squares: 16 (fp32) or 32 (bf16) of them are added in fp32, as two sums, and these go to a double.  Where that sum is not well inside

@@ -228,3 +228,21 @@ def test_norm_of_nothing_can_be_captured():
         norm = grad_norm(empty)
     graph.replay()
     assert norm.is_cuda and float(norm) == 0.0 and float(grad_norm([])) == 0.0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 3, 7, 8, 9, 8192, 16384, 16391, 100003])
+def test_views_of_a_flat_buffer(n, dtype):
+    """Every distance from a 16-byte boundary; what lies before and behind a view is neither counted nor written."""
+    from hawk_b200 import grad_norm, ops
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for off in range(8):
+        flat = torch.full((n + 24,), float("nan"), device="cuda", dtype=dtype)
+        v = flat[off:off + n]
+        v.copy_(torch.randn(n, generator=g, device="cuda"))
+        want = v.double()
+        assert abs(float(grad_norm([v])) - float(want.norm())) <= 1e-6 * float(want.norm())
+        ops.scale_in_place([v], torch.tensor(0.37, device="cuda"))
+        half = torch.finfo(dtype).eps / 2
+        assert bool(((v.double() - want * 0.37).abs() <= (half + 2 * 2.0 ** -24) * want.abs() * 0.37).all())
+        assert bool(flat[:off].isnan().all()) and bool(flat[off + n:].isnan().all())

@@ -46,6 +46,10 @@ enum { EPI_LOGITS = 0, EPI_OUT = 1, EPI_SCORE = 2, EPI_SCORE_KEEP = 3 };
 struct EpiParams {
   int M, Nc;                 // valid rows / columns of C
   int k_per_split;           // K blocks per split (EPI_OUT); a tile index runs over tiles x splits
+  // Where the rows that count are known on the device only: their number, of M or (count_is_k) of K, from which the kernel
+  // plans its tiles anew.  Null = all.  Rows of A behind it may hold anything; rows of K up to the next block's end hold zeros.
+  const int* count;
+  int count_is_k;
   // EPI_LOGITS
   float2* stats;             // [column groups of 128, M] (max, sum exp)
   float* correct;            // [M] logit at the label
@@ -166,6 +170,13 @@ __device__ __forceinline__ void box_store(const CUtensorMap* map, const unsigned
   }
 }
 
+// The K blocks of a count of rows known on the device only, over at most `most` splits: at least one block (of zeros), none without
+struct CountedSplits {
+  int blocks, per, splits;
+  __device__ __forceinline__ CountedSplits(int n, int most)
+      : blocks(max(1, (n + BK - 1) / BK)), per((blocks + most - 1) / most), splits((blocks + per - 1) / per) {}
+};
+
 // ---------------------------------------------------------------------------------------------
 // the GEMM
 // ---------------------------------------------------------------------------------------------
@@ -177,6 +188,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_c, int K, int m_tiles, int n_tiles, int splits, EpiParams ep,
                  int* status) {
+  if (ep.count) {
+    const int n = *ep.count;
+    if (ep.count_is_k) {
+      const CountedSplits c(n, splits);
+      K = c.blocks * BK;
+      ep.k_per_split = c.per;
+      splits = c.splits;
+    } else {
+      ep.M = n;
+      m_tiles = (n + BM * MH - 1) / (BM * MH);
+    }
+  }
   using Cfg = GemmCfg<MH>;
   constexpr int KSTAGES = Cfg::STAGES, STAGE_BYTES = Cfg::STAGE_BYTES, A_BYTES = Cfg::A_BYTES, NACC = Cfg::NACC;
   extern __shared__ unsigned char smem_raw[];
@@ -466,7 +489,9 @@ static __global__ void ce_poison_on_abort_kernel(const int* __restrict__ status,
 // out = scale * sum over splits of partial [splits][n], in a fixed order; 4 elements per thread (n % 4 == 0)
 template <typename TO>
 __global__ void __launch_bounds__(256)
-split_sum_kernel(const float* __restrict__ partial, long long n, int splits, const float* __restrict__ scale, TO* __restrict__ out) {
+split_sum_kernel(const float* __restrict__ partial, long long n, int splits, const float* __restrict__ scale, const int* __restrict__ count,
+                 TO* __restrict__ out) {
+  if (count) splits = CountedSplits(*count, splits).splits;
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i >= n) return;
   float4 a = *reinterpret_cast<const float4*>(partial + i);
@@ -540,16 +565,18 @@ static GradPlan plan_grad(long long M, long long Nc, long long K) {
 
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// one gradient GEMM: `out` [M, Nc] in out_dtype, times *scale
+// one gradient GEMM: `out` [M, Nc] in out_dtype, times *scale; `count` (null = K): how many of the K rows count, on the device
 template <bool A_MN, bool B_MN>
 static int grad_gemm(const __nv_bfloat16* A, long long lda, const __nv_bfloat16* B, long long ldb, void* out, int out_dtype,
-                     const float* scale, int M, int Nc, int K, float* scratch, int* status, cudaStream_t st) {
+                     const float* scale, int M, int Nc, int K, const int* count, float* scratch, int* status, cudaStream_t st) {
   const GradPlan plan = plan_grad(M, Nc, K);
   const int splits = plan.splits;
   EpiParams ep{};
   void* C = splits > 1 ? scratch : out;
   ep.out_bf16 = splits == 1 && out_dtype == HAWK_BF16;
   ep.scale = splits > 1 ? nullptr : scale;
+  ep.count = count;
+  ep.count_is_k = 1;
   int rc = plan.mh == 2
                ? launch_gemm<EPI_OUT, 2, A_MN, B_MN>(A, lda, B, ldb, C, !ep.out_bf16, Nc, M, Nc, K, splits, ep, status, st)
                : launch_gemm<EPI_OUT, 1, A_MN, B_MN>(A, lda, B, ldb, C, !ep.out_bf16, Nc, M, Nc, K, splits, ep, status, st);
@@ -557,9 +584,9 @@ static int grad_gemm(const __nv_bfloat16* A, long long lda, const __nv_bfloat16*
   const long long n = (long long)M * Nc;
   const unsigned blocks = (unsigned)((n / 4 + 255) / 256);
   if (out_dtype == HAWK_BF16)
-    split_sum_kernel<<<blocks, 256, 0, st>>>(scratch, n, splits, scale, static_cast<__nv_bfloat16*>(out));
+    split_sum_kernel<<<blocks, 256, 0, st>>>(scratch, n, splits, scale, count, static_cast<__nv_bfloat16*>(out));
   else
-    split_sum_kernel<<<blocks, 256, 0, st>>>(scratch, n, splits, scale, static_cast<float*>(out));
+    split_sum_kernel<<<blocks, 256, 0, st>>>(scratch, n, splits, scale, count, static_cast<float*>(out));
   return launch_status();
 }
 

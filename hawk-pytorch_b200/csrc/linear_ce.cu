@@ -269,11 +269,11 @@ extern "C" int hawk_linear_ce_bwd(const void* weight, const void* act, const voi
   const auto* ab = static_cast<const __nv_bfloat16*>(a_dtype == HAWK_F32 ? static_cast<const void*>(sv + S.ab) : act);
   auto* part = static_cast<float*>(scratch);
   if (dact) {    // d act [N,H] = dprobs [N,V] . W [V,H]   : A K-major (dprobs rows), B MN-major (W's rows are the K index)
-    rc = grad_gemm<false, true>(dprobs, S.ldV, wb, H, dact, da_dtype, grad_loss, (int)N, (int)H, (int)V, part, status, st);
+    rc = grad_gemm<false, true>(dprobs, S.ldV, wb, H, dact, da_dtype, grad_loss, (int)N, (int)H, (int)V, nullptr, part, status, st);
     if (rc != HAWK_OK) return rc;
   }
   if (dweight) {  // d weight [V,H] = dprobs^T . act [N,H] : A and B MN-major (the rows of dprobs and act are the K index)
-    rc = grad_gemm<true, true>(dprobs, S.ldV, ab, H, dweight, dw_dtype, grad_loss, (int)V, (int)H, (int)N, part, status, st);
+    rc = grad_gemm<true, true>(dprobs, S.ldV, ab, H, dweight, dw_dtype, grad_loss, (int)V, (int)H, (int)N, nullptr, part, status, st);
     if (rc != HAWK_OK) return rc;
   }
   ce_poison_on_abort_kernel<<<1, 1, 0, st>>>(status, dweight, dw_dtype == HAWK_BF16, dact, da_dtype == HAWK_BF16);

@@ -1,5 +1,9 @@
 // Log probability and entropy of tokens from activations and the head's weight, x = act W^T, and both gradients.  The logits
 // are never rounded and never in memory:
+//   0. rows    those that name a token, listed in order and their activations copied together (in bf16): the products below
+//      take only them, as many as the list's length on the device says, so padding and prompts cost nothing: of 32760 rows of 2048
+//      (V32000) forward and backward take 9.7 ms all named, 5.3 with half of them left out, 1.2 with 9 of 10.  48 us with all
+//      of them named, and the scatter of d act as long again; the same launch casts an fp32 weight.
 //   1. GEMM (head_gemm.cuh) whose epilogue reduces every row's 128 columns, from the fp32 accumulators, to their maximum m_g,
 //      the sum of e = e^(x - m_g) and the sum of e (x - m_g) log2 e; the token's logit is picked out on the way.  Where a
 //      gradient is wanted it stores e, in fp16: at most 1, so its rounding is 2^-12 of a probability (2^-25 of the group's largest
@@ -13,27 +17,107 @@
 // flops, 3.1 ms at N32760 H2048 V32000 where writing and reading e takes 1):
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
 //      probability, g_lp (1 - p) as -expm1; bf16 for the products, out of place: a second backward finds e as it was.
-//   4. two GEMMs, d act = dx W and d W = dx^T act.
-// Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16: 3.13 ms without and
-// 3.23 ms with what a backward needs (1.37 / 1.33 PFLOP/s), backward 6.35 ms (1.35; dx 0.71 at 5.9 TB/s, the GEMMs 2.74 and 2.80),
-// 10.9 to 11.3 ms together in a sustained loop.  At small H the logits' epilogue sets the pace: H512 N3108 97 us without, 118 with
-// (0.06 of MMAs).
+//   4. two GEMMs, d act = dx W and d W = dx^T act; d act's rows go back to their places.
+// Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16, all rows named:
+// 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.36 ms (1.35; dx 0.71 at 5.9 TB/s, the
+// GEMMs 2.74 and 2.80), 10.3 ms together in a sustained loop with a tenth left out.  At small H the logits' epilogue sets the pace:
+// H512 N3108 118 us without, 136 with (0.06 of MMAs).
 #include "head_gemm.cuh"
 
 namespace hawk {
 
+// What the forward finds out about its rows, on the device
+struct ScoreRows {
+  int* count;        // how many name a token: the compact rows 0 .. count - 1 below
+  int* row;          // [N] compact row -> row
+  int64_t* token;    // [N] compact row -> token (>= 0)
+};
+// compact rows up to here have to be zeros in the d W product, whose K blocks are of BK rows
+__device__ __forceinline__ int padded_count(int count, int N) { return min(N, (max(count, 1) + BK - 1) / BK * BK); }
+
+// The first row_blocks blocks list `per` rows each (at most one to a thread): a block counts the named tokens before its own by
+// itself, so there is no second launch and no order between blocks (N^2 / per 8-byte reads from L2 in all: 75 MB at N = 32760, of
+// the 270 that are copied).  The other blocks cast the weight.
+template <typename T>
 __global__ void __launch_bounds__(256)
-score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ correct, const int64_t* __restrict__ tokens,
-                    const __nv_bfloat16* __restrict__ weight, const __nv_bfloat16* __restrict__ act, float* __restrict__ logprob,
+score_prepare_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ act, ScoreRows rows, __nv_bfloat16* __restrict__ compact,
+                     float* __restrict__ correct, float* __restrict__ logprob, float* __restrict__ entropy, int N, int H, int per,
+                     int row_blocks, const float* __restrict__ weight, __nv_bfloat16* __restrict__ wb, long long wvec) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if ((int)blockIdx.x >= row_blocks) {
+    const long long at = ((long long)blockIdx.x - row_blocks) * 1024 + tid;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const long long i = at + q * 256;
+      if (i < wvec) {
+        float v[8];
+        VecIO<float, 8>::load(weight + i * 8, v);
+        VecIO<__nv_bfloat16, 8>::store(wb + i * 8, v);
+      }
+    }
+    return;
+  }
+  __shared__ int sums[2][8], source[256];
+  const int first = blockIdx.x * per, own = min(per, N - first);
+  int before = 0;
+#pragma unroll 8
+  for (int i = tid; i < first; i += 256) before += __ldg(tokens + i) >= 0;
+  before = __reduce_add_sync(0xffffffffu, before);
+  const int64_t token = tid < own ? __ldg(tokens + first + tid) : -1;
+  const uint32_t named = __ballot_sync(0xffffffffu, token >= 0);
+  if (lane == 0) {
+    sums[0][warp] = before;
+    sums[1][warp] = __popc(named);
+  }
+  __syncthreads();
+  before = 0;
+  int at = __popc(named & ((1u << lane) - 1)), total = 0;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) {
+    before += sums[0][w];
+    total += sums[1][w];
+    if (w < warp) at += sums[1][w];
+  }
+  if (tid < own) {
+    const int row = first + tid;
+    correct[row] = __int_as_float(0x7fc00000);  // a token >= V is in no tile: its logit stays this NaN
+    if (token >= 0) {
+      rows.row[before + at] = row;
+      rows.token[before + at] = token;
+      source[at] = row;
+    } else {
+      logprob[row] = entropy[row] = 0.f;
+    }
+  }
+  if (tid == 0 && first + own == N) *rows.count = before + total;
+  __syncthreads();
+  const int vecs = H / 8, all = total * vecs;
+#pragma unroll 4
+  for (int i = tid; i < all; i += 256) {
+    const int r = i / vecs, c = (i - r * vecs) * 8;
+    float v[8];
+    VecIO<T, 8>::load(act + (long long)source[r] * H + c, v);
+    VecIO<__nv_bfloat16, 8>::store(compact + (long long)(before + r) * H + c, v);
+  }
+}
+
+// a warp to a compact row; `act` compact, and zeroed behind the last one as far as the d W product reads
+__global__ void __launch_bounds__(256)
+score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ correct, ScoreRows rows,
+                    const __nv_bfloat16* __restrict__ weight, __nv_bfloat16* __restrict__ act, float* __restrict__ logprob,
                     float* __restrict__ entropy, float2* __restrict__ stats, int N, int H, int V, int groups,
                     const int* __restrict__ status) {
-  const int row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (row >= N) return;
-  const float4* g = score + (long long)row * groups;
-  const int64_t token = tokens[row];
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, count = *rows.count;
+  if (r >= count) {
+    if (r < padded_count(count, N))
+      for (int i = lane * 8; i < H; i += 256) *reinterpret_cast<uint4*>(act + (long long)r * H + i) = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const float4* g = score + (long long)r * groups;
+  const int64_t token = rows.token[r];
   float own = 0.f;
-  if (token >= 0 && token < V) {
-    const __nv_bfloat16 *a = act + (long long)row * H, *w = weight + token * H;
+  if (token < V) {
+    const __nv_bfloat16 *a = act + (long long)r * H, *w = weight + token * H;
 #pragma unroll 4
     for (int i = lane * 8; i < H; i += 256) {
       float av[8], wv[8];
@@ -63,8 +147,8 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
   }
   if (lane == 0) {
     const float nan = __int_as_float(0x7fc00000);
-    if (token >= 0 && token < V) {
-      const float t0 = (correct[row] - m) * kLog2e, t1 = (own - m) * kLog2e, e0 = ex2_approx(t0), e1 = ex2_approx(t1);
+    if (token < V) {
+      const float t0 = (correct[r] - m) * kLog2e, t1 = (own - m) * kLog2e, e0 = ex2_approx(t0), e1 = ex2_approx(t1);
       s = (s - e0) + e1;
       sx = (sx - e0 * t0) + e1 * t1;
     } else {
@@ -72,32 +156,34 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
     }
     const float logs = logf(s);
     float lp = (own - m) - logs, ent = logs - 0.6931471805599453f * sx / s;
-    if (token < 0) lp = ent = 0.f;
     if (*status != 0) lp = ent = nan;  // a GEMM gave up a wait (this call's, or an earlier one nobody has looked at)
-    logprob[row] = lp;
-    entropy[row] = ent;
-    stats[row] = make_float2(m, logs);
+    logprob[rows.row[r]] = lp;
+    entropy[rows.row[r]] = ent;
+    stats[r] = make_float2(m, logs);
   }
 }
 
 constexpr int kDxThreads = 512;
-// d x of one row per block, 8 columns (16 bytes of e, of one group) per thread and step
+// d x of one compact row per block, 8 columns (16 bytes of e, of one group) per thread and step
 __global__ void __launch_bounds__(kDxThreads)
 score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
-                const float* __restrict__ logprob, const float* __restrict__ entropy, const int64_t* __restrict__ tokens,
-                const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, long long ld, int V,
-                int groups) {
-  const long long row = blockIdx.x;
-  const int64_t token = tokens[row];
+                const float* __restrict__ logprob, const float* __restrict__ entropy, ScoreRows rows,
+                const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, long long ld, int N,
+                int V, int groups) {
+  const long long r = blockIdx.x;
+  const int count = *rows.count;
   const int nvec = (V + 7) / 8;  // ld is a multiple of 8; what lies behind V is never read
-  __nv_bfloat16* out = dx + row * ld;
-  if (token < 0) {
+  __nv_bfloat16* out = dx + r * ld;
+  if (r >= count) {
+    if (r >= padded_count(count, N)) return;
     for (int i = threadIdx.x; i < nvec; i += kDxThreads) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
-  const __half* in = e + row * ld;
-  const float4* g = score + row * groups;
-  const float2 st = stats[row];
+  const int row = rows.row[r];
+  const int64_t token = rows.token[r];
+  const __half* in = e + r * ld;
+  const float4* g = score + r * groups;
+  const float2 st = stats[r];
   const float lp = logprob[row], H = entropy[row], gl = g_lp ? g_lp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
   const bool known = token < V;
 #pragma unroll 4
@@ -129,29 +215,64 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   }
 }
 
-// act with the left-out rows zeroed: d x is 0 there, but 0 times what they hold need not be
+// d act from its compact rows: the sum over the splits of K, to the rows that they belong to, and zeros to the others.  A warp to 1024
+// columns of a row, 4 vectors of 8 to a lane.  N32760 H2048 in bf16 48 us (a thread to a vector, which divides 64-bit numbers: 68)
+constexpr int kScatterVecs = 4;
+template <typename TC, typename TO>
 __global__ void __launch_bounds__(256)
-keep_rows_kernel(const __nv_bfloat16* __restrict__ act, const int64_t* __restrict__ tokens, __nv_bfloat16* __restrict__ out, long long vectors,
-                 int per_row) {
-  for (long long i = (long long)blockIdx.x * 1024 + threadIdx.x, end = min(vectors, (long long)(blockIdx.x + 1) * 1024); i < end; i += 256)
-    reinterpret_cast<uint4*>(out)[i] =
-        tokens[i / per_row] < 0 ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4*>(act) + i);
+score_scatter_kernel(const TC* __restrict__ part, int splits, const int64_t* __restrict__ tokens, ScoreRows rows, TO* __restrict__ out,
+                     uint32_t units, uint32_t chunks, int N, int H) {
+  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (unit >= units) return;
+  const int r = (int)(unit / chunks), c0 = ((int)(unit - r * chunks) * 32 * kScatterVecs + (threadIdx.x & 31)) * 8;
+  const bool mine = r < *rows.count;
+  if (tokens[r] < 0) {
+    const float zero[8] = {};
+#pragma unroll
+    for (int q = 0; q < kScatterVecs; ++q)
+      if (c0 + q * 256 < H) VecIO<TO, 8>::store(out + (long long)r * H + c0 + q * 256, zero);
+  }
+  if (!mine) return;
+  float v[kScatterVecs][8];
+  const TC* in = part + (long long)r * H + c0;
+#pragma unroll
+  for (int q = 0; q < kScatterVecs; ++q)
+    if (c0 + q * 256 < H) VecIO<TC, 8>::load(in + q * 256, v[q]);
+  for (int s = 1; s < splits; ++s) {
+    in += (long long)N * H;
+#pragma unroll
+    for (int q = 0; q < kScatterVecs; ++q)
+      if (c0 + q * 256 < H) {
+        float u[8];
+        VecIO<TC, 8>::load(in + q * 256, u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[q][j] += u[j];
+      }
+  }
+  TO* to = out + (long long)rows.row[r] * H + c0;
+#pragma unroll
+  for (int q = 0; q < kScatterVecs; ++q)
+    if (c0 + q * 256 < H) VecIO<TO, 8>::store(to + q * 256, v[q]);
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
-// What the forward leaves: bf16 copies of fp32 operands, the groups' statistics and the rows', e (only for a backward)
+// What the forward leaves: the rows that name a token, their activations, an fp32 weight in bf16, the groups' statistics and the
+// rows', e (only for a backward)
 struct ScoreSaved {
-  size_t wb, ab, score, stats, correct, e, total;
+  size_t wb, ab, count, row, token, score, stats, correct, e, total;
   long long ldV;
   int groups;
 };
-static ScoreSaved score_saved(long long N, long long H, long long V, int w_dtype, int a_dtype, bool keep) {
+static ScoreSaved score_saved(long long N, long long H, long long V, int w_dtype, bool keep) {
   ScoreSaved L;
   L.ldV = (V + 7) & ~7LL;
   L.groups = (int)((V + EPI_COLS - 1) / EPI_COLS);
   size_t o = 0;
   L.wb = o;      o += w_dtype == HAWK_F32 ? up256((size_t)V * H * 2) : 0;
-  L.ab = o;      o += a_dtype == HAWK_F32 ? up256((size_t)N * H * 2) : 0;
+  L.ab = o;      o += up256((size_t)N * H * 2);
+  L.count = o;   o += 256;
+  L.row = o;     o += up256((size_t)N * 4);
+  L.token = o;   o += up256((size_t)N * 8);
   L.score = o;   o += up256((size_t)N * L.groups * sizeof(float4));
   L.stats = o;   o += up256((size_t)N * sizeof(float2));
   L.correct = o; o += up256((size_t)N * 4);
@@ -159,15 +280,18 @@ static ScoreSaved score_saved(long long N, long long H, long long V, int w_dtype
   L.total = o;
   return L;
 }
+static ScoreRows score_rows(const ScoreSaved& S, const void* saved) {
+  auto* p = const_cast<unsigned char*>(static_cast<const unsigned char*>(saved));
+  return ScoreRows{reinterpret_cast<int*>(p + S.count), reinterpret_cast<int*>(p + S.row), reinterpret_cast<int64_t*>(p + S.token)};
+}
 struct ScoreScratch {
-  size_t dx, act, partial, total;
+  size_t dx, partial, total;
 };
-static ScoreScratch score_scratch(long long N, long long H, long long V, int a_dtype, bool want_dw, bool want_da) {
+static ScoreScratch score_scratch(long long N, long long H, long long V, bool want_dw, bool want_da) {
   ScoreScratch L;
   size_t o = 0, part = 0;
   L.dx = o;      o += up256((size_t)N * ((V + 7) & ~7LL) * 2);
-  L.act = o;     o += want_dw ? up256((size_t)N * H * 2) : 0;
-  if (want_da && plan_grad(N, H, V).splits > 1) part = (size_t)plan_grad(N, H, V).splits * N * H * 4;
+  if (want_da) part = (size_t)plan_grad(N, H, V).splits * N * H * 4;  // its compact rows, in fp32 at most
   if (want_dw && plan_grad(V, H, N).splits > 1) part = std::max<size_t>(part, (size_t)plan_grad(V, H, N).splits * V * H * 4);
   L.partial = o; o += up256(part);
   L.total = o;
@@ -187,23 +311,24 @@ using namespace hawk;
 
 extern "C" size_t hawk_linear_logprobs_saved_bytes(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_grad) {
   if (N < 1 || H < 1 || V < 1) return 0;
-  return score_saved(N, H, V, w_dtype, a_dtype, want_grad != 0).total;
+  (void)a_dtype;
+  return score_saved(N, H, V, w_dtype, want_grad != 0).total;
 }
 
 extern "C" size_t hawk_linear_logprobs_scratch_bytes(int64_t N, int64_t H, int64_t V, int a_dtype, int want_dw, int want_da) {
   if (N < 1 || H < 1 || V < 1) return 0;
-  return score_scratch(N, H, V, a_dtype, want_dw != 0, want_da != 0).total;
+  (void)a_dtype;
+  return score_scratch(N, H, V, want_dw != 0, want_da != 0).total;
 }
 
-// the forward (want_dw = want_da = 0): a cast per fp32 operand, the GEMM and the reduction; the backward: d x, the copy of act, a
-// GEMM and where K is split a sum for each gradient, the look at the status word
+// the forward (want_dw = want_da = 0): the rows and casts, the GEMM and the reduction; the backward: d x, a GEMM and the scatter or,
+// where K is split, the sum for each gradient, the look at the status word
 extern "C" int hawk_linear_logprobs_kernels(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_dw, int want_da) {
+  (void)w_dtype;
+  (void)a_dtype;
   if (N < 1 || H < 1 || V < 1) return 0;
-  if (!want_dw && !want_da) return (w_dtype == HAWK_F32) + (a_dtype == HAWK_F32) + 2;
-  int n = 2;
-  if (want_dw) n += plan_grad(V, H, N).splits > 1 ? 3 : 2;
-  if (want_da) n += plan_grad(N, H, V).splits > 1 ? 2 : 1;
-  return n;
+  if (!want_dw && !want_da) return 3;
+  return 2 + (want_da ? 2 : 0) + (want_dw ? (plan_grad(V, H, N).splits > 1 ? 2 : 1) : 0);
 }
 
 extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const int64_t* tokens, float* logprob, float* entropy, void* saved,
@@ -212,42 +337,42 @@ extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const i
   HAWK_REQUIRE(weight && act && tokens && logprob && entropy && status, HAWK_ERR_NULL);
   int rc = check_score(N, H, V, w_dtype, a_dtype);
   if (rc != HAWK_OK) return rc;
-  const ScoreSaved S = score_saved(N, H, V, w_dtype, a_dtype, want_grad != 0);
+  const ScoreSaved S = score_saved(N, H, V, w_dtype, want_grad != 0);
   HAWK_REQUIRE(saved && saved_bytes >= S.total, HAWK_ERR_WORKSPACE);
   HAWK_REQUIRE(aligned(saved, 256) && aligned(weight, 16) && aligned(act, 16) && aligned(tokens, 8) && aligned(logprob, 4) &&
                    aligned(entropy, 4),
                HAWK_ERR_ALIGN);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto* sv = static_cast<unsigned char*>(saved);
-  const __nv_bfloat16* wb = static_cast<const __nv_bfloat16*>(weight);
-  const __nv_bfloat16* ab = static_cast<const __nv_bfloat16*>(act);
-  if (w_dtype == HAWK_F32) {
-    rc = hawk_cast_f32_bf16(static_cast<const float*>(weight), sv + S.wb, V * H, stream);
-    if (rc != HAWK_OK) return rc;
-    wb = reinterpret_cast<const __nv_bfloat16*>(sv + S.wb);
-  }
-  if (a_dtype == HAWK_F32) {
-    rc = hawk_cast_f32_bf16(static_cast<const float*>(act), sv + S.ab, N * H, stream);
-    if (rc != HAWK_OK) return rc;
-    ab = reinterpret_cast<const __nv_bfloat16*>(sv + S.ab);
-  }
-  // a token outside [0, V) is in no tile: its logit stays this NaN
+  const ScoreRows rows = score_rows(S, saved);
+  auto* ab = reinterpret_cast<__nv_bfloat16*>(sv + S.ab);
+  auto* wcopy = reinterpret_cast<__nv_bfloat16*>(sv + S.wb);
+  const auto* wb = w_dtype == HAWK_F32 ? wcopy : static_cast<const __nv_bfloat16*>(weight);
   auto* correct = reinterpret_cast<float*>(sv + S.correct);
-  if (cudaMemsetAsync(correct, 0xFF, (size_t)N * sizeof(float), st) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return HAWK_ERR_LAUNCH;
-  }
+  const int per = (int)std::min<int64_t>(256, std::max<int64_t>(8, (N + 4 * sm_count() - 1) / (4 * sm_count())));  // 4 blocks to an SM
+  const int64_t row_blocks = (N + per - 1) / per, wvec = w_dtype == HAWK_F32 ? V * H / 8 : 0, blocks = row_blocks + (wvec + 1023) / 1024;
+  HAWK_REQUIRE(blocks < (1LL << 31) && (int64_t)per * H < (1LL << 31), HAWK_ERR_SHAPE);
+  const auto* wf = static_cast<const float*>(weight);
+  if (a_dtype == HAWK_F32)
+    score_prepare_kernel<<<(unsigned)blocks, 256, 0, st>>>(tokens, static_cast<const float*>(act), rows, ab, correct, logprob, entropy, (int)N,
+                                                           (int)H, per, (int)row_blocks, wf, wcopy, wvec);
+  else
+    score_prepare_kernel<<<(unsigned)blocks, 256, 0, st>>>(tokens, static_cast<const __nv_bfloat16*>(act), rows, ab, correct, logprob, entropy,
+                                                           (int)N, (int)H, per, (int)row_blocks, wf, wcopy, wvec);
+  rc = launch_status();
+  if (rc != HAWK_OK) return rc;
   EpiParams ep{};
   ep.score = reinterpret_cast<float4*>(sv + S.score);
   ep.groups = S.groups;
   ep.correct = correct;
-  ep.labels = reinterpret_cast<const long long*>(tokens);
+  ep.labels = reinterpret_cast<const long long*>(rows.token);
+  ep.count = rows.count;
   if (want_grad)
     rc = launch_gemm<EPI_SCORE_KEEP, 1, false, false>(ab, H, wb, H, sv + S.e, false, S.ldV, (int)N, (int)V, (int)H, 1, ep, status, st);
   else
     rc = launch_gemm<EPI_SCORE, 1, false, false>(ab, H, wb, H, nullptr, false, S.ldV, (int)N, (int)V, (int)H, 1, ep, status, st);
   if (rc != HAWK_OK) return rc;
-  score_reduce_kernel<<<(unsigned)((N + 7) / 8), 256, 0, st>>>(ep.score, correct, tokens, wb, ab, logprob, entropy,
+  score_reduce_kernel<<<(unsigned)((N + 7) / 8), 256, 0, st>>>(ep.score, correct, rows, wb, ab, logprob, entropy,
                                                                reinterpret_cast<float2*>(sv + S.stats), (int)N, (int)H, (int)V, S.groups,
                                                                status);
   return launch_status();
@@ -261,9 +386,10 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   HAWK_REQUIRE(valid_dtype(dw_dtype) && valid_dtype(da_dtype), HAWK_ERR_DTYPE);
   int rc = check_score(N, H, V, w_dtype, a_dtype);
   if (rc != HAWK_OK) return rc;
-  const ScoreSaved S = score_saved(N, H, V, w_dtype, a_dtype, true);
-  const ScoreScratch L = score_scratch(N, H, V, a_dtype, dweight != nullptr, dact != nullptr);
+  const ScoreSaved S = score_saved(N, H, V, w_dtype, true);
+  const ScoreScratch L = score_scratch(N, H, V, dweight != nullptr, dact != nullptr);
   HAWK_REQUIRE(saved && saved_bytes >= S.total && scratch && scratch_bytes >= L.total, HAWK_ERR_WORKSPACE);
+  HAWK_REQUIRE(N * (H / 1024 + 1) < (1LL << 31), HAWK_ERR_SHAPE);
   HAWK_REQUIRE(aligned(saved, 256) && aligned(scratch, 256) && aligned(dweight, 16) && aligned(dact, 16) && aligned(weight, 16) &&
                    aligned(act, 16) && aligned(tokens, 8) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(g_logprob, 4) &&
                    aligned(g_entropy, 4),
@@ -272,26 +398,37 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const auto* sv = static_cast<const unsigned char*>(saved);
   auto* sc = static_cast<unsigned char*>(scratch);
   const auto* wb = static_cast<const __nv_bfloat16*>(w_dtype == HAWK_F32 ? static_cast<const void*>(sv + S.wb) : weight);
-  const auto* ab = static_cast<const __nv_bfloat16*>(a_dtype == HAWK_F32 ? static_cast<const void*>(sv + S.ab) : act);
+  const auto* ab = reinterpret_cast<const __nv_bfloat16*>(sv + S.ab);
+  const ScoreRows rows = score_rows(S, saved);
   auto* dx = reinterpret_cast<__nv_bfloat16*>(sc + L.dx);
   auto* part = reinterpret_cast<float*>(sc + L.partial);
   score_dx_kernel<<<(unsigned)N, kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
                                                       reinterpret_cast<const float4*>(sv + S.score),
-                                                      reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, tokens, g_logprob,
-                                                      g_entropy, dx, S.ldV, (int)V, S.groups);
+                                                      reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, rows, g_logprob,
+                                                      g_entropy, dx, S.ldV, (int)N, (int)V, S.groups);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
-  if (dact) {  // d act [N,H] = dx [N,V] . W [V,H]: A K-major, B MN-major (W's rows are the K index)
-    rc = grad_gemm<false, true>(dx, S.ldV, wb, H, dact, da_dtype, nullptr, (int)N, (int)H, (int)V, part, status, st);
+  if (dact) {  // d act [N,H] = dx [N,V] . W [V,H]: A K-major, B MN-major (W's rows are the K index); compact rows
+    const GradPlan plan = plan_grad(N, H, V);
+    EpiParams ep{};
+    ep.out_bf16 = plan.splits == 1 && da_dtype == HAWK_BF16;
+    ep.count = rows.count;
+    rc = plan.mh == 2 ? launch_gemm<EPI_OUT, 2, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, plan.splits, ep, status, st)
+                      : launch_gemm<EPI_OUT, 1, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, plan.splits, ep, status, st);
     if (rc != HAWK_OK) return rc;
-  }
-  if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the rows of dx and act are the K index)
-    auto* kept = reinterpret_cast<__nv_bfloat16*>(sc + L.act);
-    const long long vectors = N * H / 8;
-    keep_rows_kernel<<<(unsigned)((vectors + 1023) / 1024), 256, 0, st>>>(ab, tokens, kept, vectors, (int)(H / 8));
+    const int64_t chunks = (H + 256 * kScatterVecs - 1) / (256 * kScatterVecs), units = N * chunks;
+    const unsigned blocks = (unsigned)((units + 7) / 8);
+    const auto scatter = [&](const auto* from, int splits, auto* to) {
+      score_scatter_kernel<<<blocks, 256, 0, st>>>(from, splits, tokens, rows, to, (uint32_t)units, (uint32_t)chunks, (int)N, (int)H);
+    };
+    if (ep.out_bf16) scatter(reinterpret_cast<const __nv_bfloat16*>(part), 1, static_cast<__nv_bfloat16*>(dact));
+    else if (da_dtype == HAWK_BF16) scatter(static_cast<const float*>(part), plan.splits, static_cast<__nv_bfloat16*>(dact));
+    else scatter(static_cast<const float*>(part), plan.splits, static_cast<float*>(dact));
     rc = launch_status();
     if (rc != HAWK_OK) return rc;
-    rc = grad_gemm<true, true>(dx, S.ldV, kept, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)N, part, status, st);
+  }
+  if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the compact rows of dx and act are the K index)
+    rc = grad_gemm<true, true>(dx, S.ldV, ab, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)N, rows.count, part, status, st);
     if (rc != HAWK_OK) return rc;
   }
   ce_poison_on_abort_kernel<<<1, 1, 0, st>>>(status, dweight, dw_dtype == HAWK_BF16, dact, da_dtype == HAWK_BF16);

@@ -1860,9 +1860,8 @@ def linear_logprobs_fwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.T
 def _(weight, act, tokens, want_grad):
     (V, H), N = weight.shape, tokens.numel()
     up = lambda n: (n + 255) // 256 * 256  # noqa: E731
-    n = up(N * ((V + 127) // 128) * 16) + up(N * 8) + up(N * 4) + (up(N * ((V + 7) // 8 * 8) * 2) if want_grad else 0)
-    n += up(V * H * 2) if weight.dtype == torch.float32 else 0
-    n += up(N * H * 2) if act.dtype == torch.float32 else 0
+    n = up(N * ((V + 127) // 128) * 16) + 2 * up(N * 8) + 2 * up(N * 4) + 256 + (up(N * ((V + 7) // 8 * 8) * 2) if want_grad else 0)
+    n += up(N * H * 2) + (up(V * H * 2) if weight.dtype == torch.float32 else 0)
     return (*(act.new_empty(tokens.shape, dtype=torch.float32) for _ in range(2)), act.new_empty(n, dtype=torch.uint8))
 
 
@@ -1920,7 +1919,8 @@ def linear_logprobs(weight, act, tokens):
     a multiple of 8), both results fp32 of tokens' shape and differentiable in weight and act.  What fused_cross_entropy is to the
     mean loss: bf16 tensor-core products (operands in fp32 are rounded, as there), but the logits stay unrounded fp32 sums and are
     never in memory; a forward that waits for its backward holds N * V 16-bit values.  Negative tokens and those >= V as in
-    token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold."""
+    token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold, and takes no time in the
+    products (the rows that name a token are listed on the device)."""
     if weight.dim() != 2 or act.dim() < 1 or act.shape[-1] != weight.shape[1]:
         raise ValueError(f"hawk_b200: activations of shape {tuple(act.shape)} with a weight of shape {tuple(weight.shape)}")
     want = torch.is_grad_enabled() and (weight.requires_grad or act.requires_grad)

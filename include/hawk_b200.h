@@ -423,7 +423,8 @@ int hawk_token_logprobs_bwd(const void* logits, int64_t ld, const int64_t* token
  * in memory: bf16 operands (fp32 ones are rounded, as hawk_linear_ce_fwd does), fp32 sums, unrounded logits.  Negative tokens and
  * those >= V as there.  `saved` (256-byte aligned, hawk_linear_logprobs_saved_bytes) holds what the backward needs if want_grad
  * (then N*V 16-bit values among it); the backward leaves it as it is.  Gradients in dw_dtype / da_dtype, either may be NULL;
- * g_logprob, g_entropy [N] fp32, NULL = 0.  A left-out row has no part in dweight, whatever act holds there.
+ * g_logprob, g_entropy [N] fp32, NULL = 0.  A left-out row has no part in dweight, whatever act holds there, and costs next to
+ * nothing: the products run over the rows that name a token (listed on the device, nothing synchronises).
  * hawk_linear_logprobs_kernels: the forward's launches (want_dw = want_da = 0) or the backward's. */
 size_t hawk_linear_logprobs_saved_bytes(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_grad);
 size_t hawk_linear_logprobs_scratch_bytes(int64_t N, int64_t H, int64_t V, int a_dtype, int want_dw, int want_da);

@@ -209,3 +209,47 @@ def test_captured_forward_and_backward():
         x.copy_(y)
     graph.replay()
     assert all(torch.equal(x, y) for x, y in zip(out, both()))
+
+
+@pytest.mark.parametrize("N,H,V", [(600, 64, 777), (70, 32, 300), (20000, 32, 97), (5000, 512, 1000)])
+def test_any_number_of_named_rows(N, H, V):
+    """The products run over the rows that name a token alone: counts at the edges of their tiles, blocks and splits of K, in scattered
+    places, and NaN where a row is left out."""
+    w, a, t, gl, ge = _case(N, H, V, N)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for count in sorted({0, 1, 2, 63, 64, 65, 255, 256, 257, N // 2, N - 1, N}):
+        if count > N:
+            continue
+        keep = torch.randperm(N, generator=g, device="cuda")[:count]
+        some = torch.full_like(t, -1)
+        some[keep] = t[keep]
+        rows = torch.full_like(a, math.nan)
+        rows[keep] = a[keep]
+        if count:
+            lp, H_, dw, da = _check(w, rows, some, gl, ge)
+        else:
+            from hawk_b200 import linear_logprobs
+            x, y = w.detach().requires_grad_(), rows.requires_grad_()
+            lp, H_ = linear_logprobs(x, y, some)
+            dw, da = torch.autograd.grad((lp, H_), (x, y), (gl, ge))
+            assert float(dw.abs().max()) == 0
+        out = some < 0
+        assert all(bool((x[out] == 0).all()) for x in (lp, H_, da))
+
+
+def test_replays_with_other_masks():
+    from hawk_b200 import ops
+    w, a, t, gl, ge = _case(300, 64, 400, 15)
+
+    def both():
+        lp, H, saved = ops.linear_logprobs_fwd(w, a, t, True)
+        return (lp, H, *ops.linear_logprobs_bwd(w, a, t, saved, lp, H, gl, ge, True, True))
+    both()
+    torch.cuda.synchronize()
+    full, graph = t.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both()
+    for share in (0.0, 0.1, 0.9, 1.0, 0.5):
+        t.copy_(torch.where(torch.arange(300, device="cuda") * 7 % 300 < share * 300, -1, full))
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(out, both()))

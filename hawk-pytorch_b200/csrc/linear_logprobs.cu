@@ -19,7 +19,7 @@
 //      probability, g_lp (1 - p) as -expm1; bf16 for the products, out of place: a second backward finds e as it was.
 //   4. two GEMMs, d act = dx W and d W = dx^T act; d act's rows go back to their places.
 // Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16, all rows named:
-// 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.36 ms (1.35; dx 0.71 at 5.9 TB/s, the
+// 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.3 ms (1.36; dx 0.68 at 6.2 TB/s, the
 // GEMMs 2.74 and 2.80), 10.3 ms together in a sustained loop with a tenth left out.  At small H the logits' epilogue sets the pace:
 // H512 N3108 118 us without, 136 with (0.06 of MMAs).
 #include "head_gemm.cuh"
@@ -163,56 +163,70 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
   }
 }
 
-constexpr int kDxThreads = 512;
-// d x of one compact row per block, 8 columns (16 bytes of e, of one group) per thread and step
+// d x of a share of one compact row per block, 8 columns (16 bytes of e, of one group) per vector, all of a thread's requested before
+// what the row's factors are known, pairs of fp32 operations, and no call in the loop.  16380 rows of 32000: 337 us (6.2 TB/s), 1548 rows 34;
+// a row to a block of 512 threads in a loop with the token's element among the others 403 and 42
+constexpr int kDxThreads = 256, kDxVectors = 4, kDxShare = kDxThreads * kDxVectors;
 __global__ void __launch_bounds__(kDxThreads)
 score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
                 const float* __restrict__ logprob, const float* __restrict__ entropy, ScoreRows rows,
                 const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, long long ld, int N,
-                int V, int groups) {
-  const long long r = blockIdx.x;
-  const int count = *rows.count;
+                int V, int groups, uint32_t shares) {
+  const uint32_t r = blockIdx.x / shares;
+  const int i0 = (int)(blockIdx.x - r * shares) * kDxShare + (int)threadIdx.x;
   const int nvec = (V + 7) / 8;  // ld is a multiple of 8; what lies behind V is never read
+  const uint4* in = reinterpret_cast<const uint4*>(e + r * ld);
+  const float4* g = score + (long long)r * groups;
   __nv_bfloat16* out = dx + r * ld;
-  if (r >= count) {
-    if (r >= padded_count(count, N)) return;
-    for (int i = threadIdx.x; i < nvec; i += kDxThreads) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+  const int count = *rows.count;
+  if ((int)r >= count) {
+    if ((int)r >= padded_count(count, N)) return;
+#pragma unroll
+    for (int q = 0; q < kDxVectors; ++q)
+      if (i0 + q * kDxThreads < nvec) reinterpret_cast<uint4*>(out)[i0 + q * kDxThreads] = make_uint4(0u, 0u, 0u, 0u);
     return;
+  }
+  uint4 raw[kDxVectors];
+  float mg[kDxVectors];
+#pragma unroll
+  for (int q = 0; q < kDxVectors; ++q) {
+    const int i = i0 + q * kDxThreads;
+    if (i < nvec) {
+      raw[q] = __ldg(in + i);
+      mg[q] = __ldg(&g[i / (EPI_COLS / 8)].x);
+    }
   }
   const int row = rows.row[r];
   const int64_t token = rows.token[r];
-  const __half* in = e + r * ld;
-  const float4* g = score + r * groups;
   const float2 st = stats[r];
   const float lp = logprob[row], H = entropy[row], gl = g_lp ? g_lp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
   const bool known = token < V;
-#pragma unroll 4
-  for (int i = threadIdx.x; i < nvec; i += kDxThreads) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(in) + i);
-    const float off = (__ldg(&g[i / (EPI_COLS / 8)].x) - st.x) - st.y;  // log p of the group's maximum
-    const float f = known ? ex2_approx(off * kLog2e) : __int_as_float(0x7fc00000);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int q = 0; q < kDxVectors; ++q) {
+    const int i = i0 + q * kDxThreads;
+    if (i >= nvec) break;
+    const float off = (mg[q] - st.x) - st.y;  // log p of the group's maximum
+    const float2 f = f2(known ? -ex2_approx(off * kLog2e) : __int_as_float(0x7fc00000)), k0 = f2(off + H);
+    const uint32_t w[4] = {raw[q].x, raw[q].y, raw[q].z, raw[q].w};
     float d[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 ev = unpack_f16x2(w[q]);
-      float c0 = gl, c1 = gl;
-      if (gh != 0.f) {  // the same for all of the row
-        c0 = fmaf(gh, fmaf(fmaxf(__log2f(ev.x), -200.f), 0.6931471805599453f, off) + H, gl);  // e = 0: a finite factor
-        c1 = fmaf(gh, fmaf(fmaxf(__log2f(ev.y), -200.f), 0.6931471805599453f, off) + H, gl);
+    for (int k = 0; k < 4; ++k) {
+      const float2 ev = unpack_f16x2(w[k]);
+      float2 c = f2(gl);
+      if (gh != 0.f) {  // the same for all of the row.  2^-40: a finite factor where e = 0, nothing to the others (2^-24 at least)
+        const float2 l = add2(ev, f2(0x1p-40f));
+        c = fma2(f2(gh), fma2(make_float2(__log2f(l.x), __log2f(l.y)), f2(0.6931471805599453f), k0), c);
       }
-      d[2 * q] = -ev.x * f * c0;
-      d[2 * q + 1] = -ev.y * f * c1;
-    }
-    const int64_t at = token - (int64_t)i * 8;
-    if (at >= 0 && at < 8) {
-      const float own = fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H));
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j == (int)at) d[j] = own;
+      c = mul2(mul2(ev, f), c);
+      d[2 * k] = c.x;
+      d[2 * k + 1] = c.y;
     }
     VecIO<__nv_bfloat16, 8>::store(out + (long long)i * 8, d);
   }
+  // the token's own element anew, by the thread that wrote it
+  const int64_t in_share = token / 8 - (i0 - (int)threadIdx.x);
+  if (known && in_share >= 0 && in_share < kDxShare && (int)threadIdx.x == (int)in_share % kDxThreads)
+    out[token] = __float2bfloat16(fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H)));
 }
 
 // d act from its compact rows: the sum over the splits of K, to the rows that they belong to, and zeros to the others.  A warp to 1024
@@ -389,7 +403,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const ScoreSaved S = score_saved(N, H, V, w_dtype, true);
   const ScoreScratch L = score_scratch(N, H, V, dweight != nullptr, dact != nullptr);
   HAWK_REQUIRE(saved && saved_bytes >= S.total && scratch && scratch_bytes >= L.total, HAWK_ERR_WORKSPACE);
-  HAWK_REQUIRE(N * (H / 1024 + 1) < (1LL << 31), HAWK_ERR_SHAPE);
+  HAWK_REQUIRE(N * (H / 1024 + 1) < (1LL << 31) && N * (V / (8 * kDxShare) + 1) < (1LL << 31), HAWK_ERR_SHAPE);
   HAWK_REQUIRE(aligned(saved, 256) && aligned(scratch, 256) && aligned(dweight, 16) && aligned(dact, 16) && aligned(weight, 16) &&
                    aligned(act, 16) && aligned(tokens, 8) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(g_logprob, 4) &&
                    aligned(g_entropy, 4),
@@ -402,10 +416,12 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const ScoreRows rows = score_rows(S, saved);
   auto* dx = reinterpret_cast<__nv_bfloat16*>(sc + L.dx);
   auto* part = reinterpret_cast<float*>(sc + L.partial);
-  score_dx_kernel<<<(unsigned)N, kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
-                                                      reinterpret_cast<const float4*>(sv + S.score),
-                                                      reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, rows, g_logprob,
-                                                      g_entropy, dx, S.ldV, (int)N, (int)V, S.groups);
+  const int64_t shares = ((V + 7) / 8 + kDxShare - 1) / kDxShare;
+  score_dx_kernel<<<(unsigned)(N * shares), kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
+                                                                 reinterpret_cast<const float4*>(sv + S.score),
+                                                                 reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, rows,
+                                                                 g_logprob, g_entropy, dx, S.ldV, (int)N, (int)V, S.groups,
+                                                                 (uint32_t)shares);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
   if (dact) {  // d act [N,H] = dx [N,V] . W [V,H]: A K-major, B MN-major (W's rows are the K index); compact rows

@@ -36,13 +36,21 @@ struct ScoreRows {
 __device__ __forceinline__ int padded_count(int count, int N) { return min(N, (max(count, 1) + BK - 1) / BK * BK); }
 
 // The first row_blocks blocks list `per` rows each (at most one to a thread): a block counts the named tokens before its own by
-// itself, so there is no second launch and no order between blocks (N^2 / per 8-byte reads from L2 in all: 75 MB at N = 32760, of
-// the 270 that are copied).  The other blocks cast the weight.
+// itself, so there is no second launch and no order between blocks.  That is N^2 / (2 per) tokens read from L2 in all: 75 MB at
+// N = 32760, of the 270 that are copied, but 64 ms at 10 M rows; longer lists are counted by block first (`counts`, null otherwise) and
+// a block adds up the counts before its own.  The other blocks cast the weight.
+constexpr int64_t kCountedRows = 32768;
+__global__ void __launch_bounds__(256) score_count_kernel(const int64_t* __restrict__ tokens, int* __restrict__ counts, int N, int per) {
+  const int row = blockIdx.x * per + threadIdx.x;
+  const int n = __syncthreads_count((int)threadIdx.x < per && row < N && __ldg(tokens + min(row, N - 1)) >= 0);
+  if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256)
 score_prepare_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ act, ScoreRows rows, __nv_bfloat16* __restrict__ compact,
                      float* __restrict__ correct, float* __restrict__ logprob, float* __restrict__ entropy, int N, int H, int per,
-                     int row_blocks, const float* __restrict__ weight, __nv_bfloat16* __restrict__ wb, long long wvec) {
+                     int row_blocks, const int* __restrict__ counts, const float* __restrict__ weight, __nv_bfloat16* __restrict__ wb, long long wvec) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((int)blockIdx.x >= row_blocks) {
     const long long at = ((long long)blockIdx.x - row_blocks) * 1024 + tid;
@@ -60,8 +68,13 @@ score_prepare_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ a
   __shared__ int sums[2][8], source[256];
   const int first = blockIdx.x * per, own = min(per, N - first);
   int before = 0;
+  if (counts) {
 #pragma unroll 8
-  for (int i = tid; i < first; i += 256) before += __ldg(tokens + i) >= 0;
+    for (int i = tid; i < (int)blockIdx.x; i += 256) before += __ldg(counts + i);
+  } else {
+#pragma unroll 8
+    for (int i = tid; i < first; i += 256) before += __ldg(tokens + i) >= 0;
+  }
   before = __reduce_add_sync(0xffffffffu, before);
   const int64_t token = tid < own ? __ldg(tokens + first + tid) : -1;
   const uint32_t named = __ballot_sync(0xffffffffu, token >= 0);
@@ -335,13 +348,13 @@ extern "C" size_t hawk_linear_logprobs_scratch_bytes(int64_t N, int64_t H, int64
   return score_scratch(N, H, V, want_dw != 0, want_da != 0).total;
 }
 
-// the forward (want_dw = want_da = 0): the rows and casts, the GEMM and the reduction; the backward: d x, a GEMM and the scatter or,
+// the forward (want_dw = want_da = 0): the rows (counted before in long lists) and casts, the GEMM and the reduction; the backward: d x, a GEMM and the scatter or,
 // where K is split, the sum for each gradient, the look at the status word
 extern "C" int hawk_linear_logprobs_kernels(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_dw, int want_da) {
   (void)w_dtype;
   (void)a_dtype;
   if (N < 1 || H < 1 || V < 1) return 0;
-  if (!want_dw && !want_da) return 3;
+  if (!want_dw && !want_da) return N > kCountedRows ? 4 : 3;
   return 2 + (want_da ? 2 : 0) + (want_dw ? (plan_grad(V, H, N).splits > 1 ? 2 : 1) : 0);
 }
 
@@ -367,12 +380,19 @@ extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const i
   const int64_t row_blocks = (N + per - 1) / per, wvec = w_dtype == HAWK_F32 ? V * H / 8 : 0, blocks = row_blocks + (wvec + 1023) / 1024;
   HAWK_REQUIRE(blocks < (1LL << 31) && (int64_t)per * H < (1LL << 31), HAWK_ERR_SHAPE);
   const auto* wf = static_cast<const float*>(weight);
+  int* counts = nullptr;
+  if (N > kCountedRows) {
+    counts = reinterpret_cast<int*>(sv + S.score);  // free until the GEMM writes it, and 16 bytes to a row at least
+    score_count_kernel<<<(unsigned)row_blocks, 256, 0, st>>>(tokens, counts, (int)N, per);
+    rc = launch_status();
+    if (rc != HAWK_OK) return rc;
+  }
   if (a_dtype == HAWK_F32)
     score_prepare_kernel<<<(unsigned)blocks, 256, 0, st>>>(tokens, static_cast<const float*>(act), rows, ab, correct, logprob, entropy, (int)N,
-                                                           (int)H, per, (int)row_blocks, wf, wcopy, wvec);
+                                                           (int)H, per, (int)row_blocks, counts, wf, wcopy, wvec);
   else
     score_prepare_kernel<<<(unsigned)blocks, 256, 0, st>>>(tokens, static_cast<const __nv_bfloat16*>(act), rows, ab, correct, logprob, entropy,
-                                                           (int)N, (int)H, per, (int)row_blocks, wf, wcopy, wvec);
+                                                           (int)N, (int)H, per, (int)row_blocks, counts, wf, wcopy, wvec);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
   EpiParams ep{};

@@ -253,3 +253,18 @@ def test_replays_with_other_masks():
         t.copy_(torch.where(torch.arange(300, device="cuda") * 7 % 300 < share * 300, -1, full))
         graph.replay()
         assert all(torch.equal(x, y) for x, y in zip(out, both()))
+
+
+@pytest.mark.parametrize("N", [32768, 32769, 100003])
+@pytest.mark.parametrize("share", [0.0, 0.3])
+def test_long_lists_of_rows(N, share):
+    """Lists on both sides of where their blocks are counted first, and the number of launches that goes with it."""
+    from hawk_b200 import ops
+    w, a, t, gl, ge = _case(N, 32, 70, 16)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    t = torch.where(torch.rand(N, generator=g, device="cuda") < share, -3, t)
+    ops.LOG.reset()
+    _check(w, a, t, gl, ge)
+    counts = dict(ops.LOG.counts)
+    ops.LOG.enabled = False
+    assert counts["linear_logprobs"] == 2 * (4 if N > 32768 else 3)

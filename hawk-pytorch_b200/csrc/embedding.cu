@@ -7,7 +7,7 @@
 // Measured (32768 tokens as frequent as in text, V32000 H2048): forward 55 us fp32 (6.2 TB/s), 29 bf16; backward 135 us fp32 of
 // 81 for its 530 MB alone, 103 bf16: group 23, windows 30, rows 83.
 //
-// Backward, three launches:
+// Backward, three launches (up to 2048 tokens one, embed_small_kernel):
 //   1. group   the positions of each id side by side, in their order (a stable counting sort).  A block owns one id in 128 (EmbedOrder)
 //              and reads all ids (from L2: 128 blocks x 8 B, against rows of kilobytes): it counts those of the blocks before it,
 //              which gives its place in the result without a word from them, and queues its own in shared memory in their order.
@@ -474,6 +474,132 @@ __global__ void __launch_bounds__(256, 3) embed_rows_kernel(const T* __restrict_
   }
 }
 
+// ---- backward of few tokens: one launch, no workspace --------------------------------------------------------
+// Up to 2048 positions (us, this against the three launches, text-like ids and in brackets one id for all; V32000): N64 H512 fp32 12
+// against 20 (14, 22), N1551 16 against 23 (57, 26: one SM reads all rows), N2048 H2048 bf16 30 against 42 (82, 42); N4096 37 against
+// 48 (150, 48) is left to the three.  Two launches and a workspace less are 15 us of the host's time.
+// A block owns the ids b, b + blocks, .. and 512 columns of their rows (256 in the scalar form).  Its warps go through an eighth of the
+// positions each and list their block's in order; then a warp to a table row adds up its positions, or writes its zeros.  Ids with more
+// than kSmallLong positions are added up by all warps, each its eighth of them, and the eight sums in order.
+constexpr int kSmallIds = 2048, kSmallSlots = 1024, kSmallLogBlocks = 9, kSmallLong = 16;
+__host__ __device__ constexpr bool few_ids(int64_t N, int64_t V) { return N <= kSmallIds && V <= (int64_t)kSmallSlots << kSmallLogBlocks; }
+
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) embed_small_kernel(const int64_t* __restrict__ ids, const T* __restrict__ dout, T* __restrict__ dw, int N,
+                                                          int V, int H, int64_t padding, float scale, int log_blocks, int share) {
+  constexpr int U = unit_vectors<T>(VEC), kRows = 32 / (U * (Raw<T, VEC>::B > 4 ? Raw<T, VEC>::B / 4 : 1));  // rows in flight
+  __shared__ uint32_t list[kSmallIds];                // slot << 16 | position, `share` words to a warp
+  __shared__ int count[kSmallSlots], found[8], longs[kSmallIds / kSmallLong], nlongs;
+  __shared__ __align__(16) float sums[8][32 * VEC * U];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.y;
+  const int slots = (V - b + (1 << log_blocks) - 1) >> log_blocks, c0 = (blockIdx.x * U * 32 + lane) * VEC;
+  for (int k = tid; k < slots; k += 256) count[k] = 0;
+  if (tid == 0) nlongs = 0;
+  __syncthreads();
+  int n = 0;
+  uint32_t* mine = list + warp * share;
+  for (int i0 = warp * share, end = min(N, i0 + share); i0 < end; i0 += 128) {
+    int64_t id[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) id[q] = i0 + q * 32 + lane < end ? __ldg(ids + i0 + q * 32 + lane) : -1;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const bool own = id[q] >= 0 && id[q] < V && id[q] != padding && ((int)id[q] & ((1 << log_blocks) - 1)) == b;
+      const uint32_t m = __ballot_sync(0xffffffffu, own);
+      if (own) {
+        const int k = (int)id[q] >> log_blocks;
+        mine[n + __popc(m & ((1u << lane) - 1))] = (uint32_t)k << 16 | (uint32_t)(i0 + q * 32 + lane);
+        atomicAdd(&count[k], 1);
+      }
+      n += __popc(m);
+    }
+  }
+  if (lane == 0) found[warp] = n;
+  __syncthreads();
+
+  float acc[U][VEC];
+  const auto clear = [&] {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) acc[u][j] = 0.f;
+  };
+  // adds the rows of the positions that lanes of `m` hold, in the lanes' order
+  const auto add = [&](uint32_t m, int position) {
+    while (m) {
+      typename Raw<T, VEC>::type v[kRows][U];
+      int have = 0;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (m) {
+          const T* row = dout + (int64_t)__shfl_sync(0xffffffffu, position, __ffs((int)m) - 1) * H;
+          m &= m - 1;
+          have = r + 1;
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + u * 32 * VEC < H) v[r][u] = Raw<T, VEC>::load(row + c0 + u * 32 * VEC);
+        }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+        if (r < have) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + u * 32 * VEC < H) {
+              float x[VEC];
+              Raw<T, VEC>::unpack(v[r][u], x);
+#pragma unroll
+              for (int j = 0; j < VEC; ++j) acc[u][j] += x[j];
+            }
+        }
+    }
+  };
+  // the positions of slot k in warp w's list
+  const auto add_list = [&](int w, int k) {
+    for (int i = 0; i < found[w]; i += 32) {
+      const uint32_t e = i + lane < found[w] ? list[w * share + i + lane] : 0xffffffffu;
+      add(__ballot_sync(0xffffffffu, e >> 16 == (uint32_t)k), (int)(e & 0xffffu));
+    }
+  };
+  for (int k = warp; k < slots; k += 8) {
+    const int c = count[k];
+    if (c > kSmallLong) {
+      if (lane == 0) longs[atomicAdd(&nlongs, 1)] = k;
+      continue;
+    }
+    clear();
+    if (c)
+      for (int w = 0; w < 8; ++w) add_list(w, k);
+    T* out = dw + ((int64_t)k << log_blocks | b) * H;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (c0 + u * 32 * VEC < H) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[u][j] *= scale;
+        VecIO<T, VEC>::store(out + c0 + u * 32 * VEC, acc[u]);
+      }
+  }
+  __syncthreads();
+  for (int l = 0; l < nlongs; ++l) {
+    const int k = longs[l];
+    clear();
+    add_list(warp, k);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) sums[warp][(u * 32 + lane) * VEC + j] = acc[u][j];
+    __syncthreads();
+    T* out = dw + ((int64_t)k << log_blocks | b) * H;
+    for (int i = tid; i < 32 * U * VEC; i += 256) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s += sums[w][i];
+      const int col = blockIdx.x * U * 32 * VEC + i;
+      if (col < H) out[col] = from_float<T>(s * scale);
+    }
+    __syncthreads();
+  }
+}
+
 // ---- host --------------------------------------------------------------------------------------------------
 static size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -500,6 +626,17 @@ static EmbedWs embed_ws(int64_t N, int64_t V, int64_t H) {
   L.runs = o;    o += N > kLong ? up256((size_t)(order.groups() + (1LL << order.log_blocks)) * sizeof(int4)) : 0;
   L.total = o;
   return L;
+}
+
+template <typename T, int VEC>
+static int embed_small(const int64_t* ids, const void* dout, void* dw, int64_t N, int64_t V, int H, int64_t padding, float scale,
+                       cudaStream_t st) {
+  int log_blocks = kSmallLogBlocks;
+  while (log_blocks > 0 && (1LL << log_blocks) > V) --log_blocks;
+  const int cols = 32 * VEC * unit_vectors<T>(VEC), chunks = (H + cols - 1) / cols, share = (int)((N + 255) / 256) * 32;
+  embed_small_kernel<T, VEC><<<dim3((unsigned)chunks, 1u << log_blocks), 256, 0, st>>>(
+      ids, static_cast<const T*>(dout), static_cast<T*>(dw), (int)N, (int)V, H, padding, scale, log_blocks, share);
+  return launch_status();
 }
 
 static int check_embed(int64_t N, int64_t V, int64_t H, int dtype) {
@@ -563,7 +700,11 @@ extern "C" int hawk_embedding_fwd(const int64_t* ids, const void* weight, void* 
 }
 
 extern "C" size_t hawk_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H) {
-  return N < 1 || V < 1 || H < 1 ? 0 : embed_ws(N, V, H).total;
+  return N < 1 || V < 1 || H < 1 || few_ids(N, V) ? 0 : embed_ws(N, V, H).total;
+}
+
+extern "C" int hawk_embedding_bwd_kernels(int64_t N, int64_t V, int64_t H) {
+  return N < 1 || V < 1 || H < 1 ? 0 : few_ids(N, V) ? 1 : N > kLong ? 3 : 2;
 }
 
 extern "C" int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dweight, void* workspace, size_t workspace_bytes, int64_t N,
@@ -571,11 +712,13 @@ extern "C" int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dw
   HAWK_REQUIRE(ids && dout && dweight, HAWK_ERR_NULL);
   const int ok = check_embed(N, V, H, dtype);
   if (ok != HAWK_OK) return ok;
-  const EmbedWs L = embed_ws(N, V, H);
-  HAWK_REQUIRE(workspace && workspace_bytes >= L.total, HAWK_ERR_WORKSPACE);
   const int es = (int)dtype_size(dtype);
   HAWK_REQUIRE(aligned(ids, 8) && aligned(dout, es) && aligned(dweight, es) && aligned(workspace, 16), HAWK_ERR_ALIGN);
+  const int vec = common_vec((int)H, es, dout, dweight);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (few_ids(N, V)) return HAWK_BY_VEC(embed_small, dtype, vec, ids, dout, dweight, N, V, (int)H, padding_idx, scale, st);
+  const EmbedWs L = embed_ws(N, V, H);
+  HAWK_REQUIRE(workspace && workspace_bytes >= L.total, HAWK_ERR_WORKSPACE);
   auto* ws = static_cast<unsigned char*>(workspace);
   auto* perm = reinterpret_cast<int*>(ws + L.perm);
   auto* start = reinterpret_cast<int*>(ws + L.start);
@@ -594,7 +737,6 @@ extern "C" int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dw
   embed_group_kernel<<<1u << order.log_blocks, kGroupThreads, smem, st>>>(ids, N, V, padding_idx, order, perm, start, owner, runs, windows, queue);
   const int rc = launch_status();
   if (rc != HAWK_OK) return rc;
-  const int vec = common_vec((int)H, es, dout, dweight);
   return HAWK_BY_VEC(embed_sums, dtype, vec, dout, dweight, perm, start, reinterpret_cast<float*>(ws + L.partial),
                      owner, runs, order, N, V, (int)H, scale, st);
 }

@@ -65,6 +65,7 @@ SIGNATURES = {
     "hawk_scale_multi": (c_int, [c_char_p, c_int, _P, _P]),
     "hawk_embedding_fwd": (c_int, [_P, _P, _P, c_int64, c_int64, c_int64, c_float, c_int, _P]),
     "hawk_embedding_bwd_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "hawk_embedding_bwd_kernels": (c_int, [c_int64, c_int64, c_int64]),
     "hawk_embedding_bwd": (c_int, [_P, _P, _P, _P, c_size_t, c_int64, c_int64, c_int64, c_int64, c_float, c_int, _P]),
     "hawk_token_logprobs": (c_int, [_P, c_int64] + [_P] * 6 + [c_int64, c_int64, c_int, c_int, _P]),
     "hawk_token_logprobs_bwd": (c_int, [_P, c_int64] + [_P] * 7 + [c_int64, c_int64, c_int, _P]),

@@ -1960,9 +1960,10 @@ def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, V: int, scale: float, p
     if N == 0 or H == 0:
         return torch.zeros(V, H, dtype=dout.dtype, device=dout.device)
     dw = torch.empty(V, H, dtype=dout.dtype, device=dout.device)
-    ws = torch.empty(lib.hawk_embedding_bwd_workspace_bytes(N, V, H), dtype=torch.uint8, device=dout.device)
-    with _on(dout, "embedding_bwd", 3 if N > 16 else 2):
-        _lib.check(lib.hawk_embedding_bwd(ids.data_ptr(), dout.data_ptr(), dw.data_ptr(), ws.data_ptr(), ws.numel(), N, V, H,
+    size = lib.hawk_embedding_bwd_workspace_bytes(N, V, H)
+    ws = torch.empty(size, dtype=torch.uint8, device=dout.device) if size else None
+    with _on(dout, "embedding_bwd", lambda: lib.hawk_embedding_bwd_kernels(N, V, H)):
+        _lib.check(lib.hawk_embedding_bwd(ids.data_ptr(), dout.data_ptr(), dw.data_ptr(), _ptr(ws), size, N, V, H,
                                           padding_idx, scale, _dt(dout), _stream(dout)), "hawk_embedding_bwd")
     return dw
 

@@ -397,10 +397,12 @@ int hawk_scale_multi(const hawk_norm_tensor* tensors, int count, const float* sc
  * out[i] = scale * weight[ids[i]]; dweight[v] = scale * sum of dout[i] over the positions i with ids[i] = v, in their order,
  * summed in fp32 and rounded once (deterministic; rows that no position names become zero).  ids [N] int64, weight, dweight
  * [V,H], out, dout [N,H] of one dtype, any H.  An id outside [0, V) gives a row of NaN and no gradient; neither does one equal
- * to padding_idx (-1: none).  Workspace (backward): 16-byte aligned, hawk_embedding_bwd_workspace_bytes. */
+ * to padding_idx (-1: none).  Workspace (backward): 16-byte aligned, hawk_embedding_bwd_workspace_bytes (0 for
+ * few tokens: NULL).  hawk_embedding_bwd_kernels: its launches. */
 int hawk_embedding_fwd(const int64_t* ids, const void* weight, void* out, int64_t N, int64_t V, int64_t H, float scale,
                        int dtype, void* stream);
 size_t hawk_embedding_bwd_workspace_bytes(int64_t N, int64_t V, int64_t H);
+int hawk_embedding_bwd_kernels(int64_t N, int64_t V, int64_t H);
 int hawk_embedding_bwd(const int64_t* ids, const void* dout, void* dweight, void* workspace, size_t workspace_bytes,
                        int64_t N, int64_t V, int64_t H, int64_t padding_idx, float scale, int dtype, void* stream);
 

@@ -70,12 +70,14 @@ def test_embedding_argument_validation():
     assert lib.hawk_embedding_fwd(p, p, p, 1 << 31, 10, 8, 1.0, 0, None) == -2
     assert lib.hawk_embedding_fwd(p, p, p, 4, 10, 8, 1.0, 5, None) == -3
     assert lib.hawk_embedding_fwd(p, ctypes.c_void_p(4098), p, 4, 10, 8, 1.0, 0, None) == -4
-    ws = lib.hawk_embedding_bwd_workspace_bytes(100, 10, 8)
+    ws = lib.hawk_embedding_bwd_workspace_bytes(5000, 10, 8)
     assert ws >= 100 * 4 + 11 * 4 + 3 * 8 * 4
-    assert lib.hawk_embedding_bwd(p, p, p, None, ws, 100, 10, 8, -1, 1.0, 0, None) == -5
-    assert lib.hawk_embedding_bwd(p, p, p, p, ws - 1, 100, 10, 8, -1, 1.0, 0, None) == -5
+    assert lib.hawk_embedding_bwd(p, p, p, None, ws, 5000, 10, 8, -1, 1.0, 0, None) == -5
+    assert lib.hawk_embedding_bwd(p, p, p, p, ws - 1, 5000, 10, 8, -1, 1.0, 0, None) == -5
     assert lib.hawk_embedding_bwd(p, p, p, ctypes.c_void_p(4100), ws, 100, 10, 8, -1, 1.0, 0, None) == -4
     assert lib.hawk_embedding_bwd(p, None, p, p, ws, 100, 10, 8, -1, 1.0, 0, None) == -1
+    assert lib.hawk_embedding_bwd_workspace_bytes(2048, 1 << 19, 8) == 0 < lib.hawk_embedding_bwd_workspace_bytes(2048, (1 << 19) + 1, 8)
+    assert [lib.hawk_embedding_bwd_kernels(*a) for a in ((2048, 10, 8), (2049, 10, 8), (16, 1 << 20, 8), (17, 1 << 20, 8))] == [1, 3, 2, 3]
 
 
 def test_embedding_refuses_cpu_tensors():

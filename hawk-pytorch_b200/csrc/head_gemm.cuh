@@ -60,6 +60,7 @@ struct EpiParams {
   // EPI_OUT
   int out_bf16;              // the store map's type
   const float* scale;        // device scalar multiplied in; null = 1
+  const float* row_scale;    // [M] factors of the rows; null = 1
 };
 
 constexpr int MN_BOX = 64 * 128;  // bytes of one [64 columns x 64 rows] box of an MN-major operand
@@ -418,6 +419,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         if (row_ok && col0 < ep.Nc) ep.stats[(long long)(col0 / EPI_COLS) * ep.M + row] = make_float2(run_m, run_s);
       } else {
         const int split = tile / tiles;
+        const float f = ep.row_scale && row_ok ? scale * __ldg(ep.row_scale + row) : scale;
         auto chunk = [&](int c) -> const uint32_t(&)[32] {  // waits for chunk c, requests the next one
           tmem_ld_wait();
           if (c + 1 < EPI_COLS / 32) tmem_ld32_async(taddr0 + (c + 1) * 32, v[(c + 1) & 1]);
@@ -430,7 +432,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             uint32_t packed[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-              packed[j] = pack_bf16x2(__uint_as_float(w[2 * j]) * scale, __uint_as_float(w[2 * j + 1]) * scale);
+              packed[j] = pack_bf16x2(__uint_as_float(w[2 * j]) * f, __uint_as_float(w[2 * j + 1]) * f);
             unsigned char* box = boxes + ((c >> 1) % Cfg::NBOX) * BOX_BYTES;
             if ((c & 1) == 0) box_reuse<Cfg::NBOX>(lane);
             box_put(box, lane, (c & 1) * 4, packed);
@@ -446,7 +448,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             for (int q = 0; q < 2; ++q) {
               uint32_t scaled[16];
 #pragma unroll
-              for (int j = 0; j < 16; ++j) scaled[j] = __float_as_uint(__uint_as_float(w[16 * q + j]) * scale);
+              for (int j = 0; j < 16; ++j) scaled[j] = __float_as_uint(__uint_as_float(w[16 * q + j]) * f);
               box_put(box, lane, q * 4, scaled);
             }
             box_store(&map_c, box, lane, col0 + c * 32, row0, split, ep);

@@ -16,10 +16,13 @@
 // Backward, from e and the groups' maxima (2 N V bytes kept instead of a third GEMM: forming the logits again takes 2 N H V
 // flops, 3.1 ms at N32760 H2048 V32000 where writing and reading e takes 1):
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
-//      probability, g_lp (1 - p) as -expm1; bf16 for the products, out of place: a second backward finds e as it was.
+//      probability, g_lp (1 - p) as -expm1; bf16 for the products, out of place: a second backward finds e as it was.  The token's
+//      element is most of its row, so the row is first scaled, by 2^-8 at most, to where that element is a bf16 number, and d act's
+//      row is scaled back as it leaves the product: its error is then that of its own rounding alone (1.7e-3 in norm where two
+//      roundings left 2.4e-3).  d W takes the rows as they are, which is the element's own rounding, as before.
 //   4. two GEMMs, d act = dx W and d W = dx^T act; d act's rows go back to their places.
 // Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16, all rows named:
-// 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.3 ms (1.36; dx 0.68 at 6.2 TB/s, the
+// 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.3 ms (1.36; dx 0.7 at 5.9 TB/s, the
 // GEMMs 2.74 and 2.80), 10.3 ms together in a sustained loop with a tenth left out.  At small H the logits' epilogue sets the pace:
 // H512 N3108 118 us without, 136 with (0.06 of MMAs).
 #include "head_gemm.cuh"
@@ -177,14 +180,14 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
 }
 
 // d x of a share of one compact row per block, 8 columns (16 bytes of e, of one group) per vector, all of a thread's requested before
-// what the row's factors are known, pairs of fp32 operations, and no call in the loop.  16380 rows of 32000: 337 us (6.2 TB/s), 1548 rows 34;
+// what the row's factors are known, pairs of fp32 operations, and no call in the loop.  16380 rows of 32000: 355 us (5.9 TB/s), 1548 rows 36;
 // a row to a block of 512 threads in a loop with the token's element among the others 403 and 42
 constexpr int kDxThreads = 256, kDxVectors = 4, kDxShare = kDxThreads * kDxVectors;
 __global__ void __launch_bounds__(kDxThreads)
 score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
                 const float* __restrict__ logprob, const float* __restrict__ entropy, ScoreRows rows,
-                const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, long long ld, int N,
-                int V, int groups, uint32_t shares) {
+                const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, float* __restrict__ row_scale,
+                long long ld, int N, int V, int groups, uint32_t shares) {
   const uint32_t r = blockIdx.x / shares;
   const int i0 = (int)(blockIdx.x - r * shares) * kDxShare + (int)threadIdx.x;
   const int nvec = (V + 7) / 8;  // ld is a multiple of 8; what lies behind V is never read
@@ -214,12 +217,16 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   const float2 st = stats[r];
   const float lp = logprob[row], H = entropy[row], gl = g_lp ? g_lp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
   const bool known = token < V;
+  const float own = fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H)), own16 = __bfloat162float(__float2bfloat16(own));
+  const bool scaled = fabsf(own) > 1e-30f && fabsf(own16) < 1e37f;
+  const float shrink = scaled ? own16 / own : 1.f;
+  if (blockIdx.x == r * shares && threadIdx.x == 0) row_scale[r] = scaled ? own / own16 : 1.f;
 #pragma unroll
   for (int q = 0; q < kDxVectors; ++q) {
     const int i = i0 + q * kDxThreads;
     if (i >= nvec) break;
     const float off = (mg[q] - st.x) - st.y;  // log p of the group's maximum
-    const float2 f = f2(known ? -ex2_approx(off * kLog2e) : __int_as_float(0x7fc00000)), k0 = f2(off + H);
+    const float2 f = f2(known ? -ex2_approx(off * kLog2e) * shrink : __int_as_float(0x7fc00000)), k0 = f2(off + H);
     const uint32_t w[4] = {raw[q].x, raw[q].y, raw[q].z, raw[q].w};
     float d[8];
 #pragma unroll
@@ -239,7 +246,7 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   // the token's own element anew, by the thread that wrote it
   const int64_t in_share = token / 8 - (i0 - (int)threadIdx.x);
   if (known && in_share >= 0 && in_share < kDxShare && (int)threadIdx.x == (int)in_share % kDxThreads)
-    out[token] = __float2bfloat16(fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H)));
+    out[token] = __float2bfloat16(own);
 }
 
 // d act from its compact rows: the sum over the splits of K, to the rows that they belong to, and zeros to the others.  A warp to 1024
@@ -312,12 +319,13 @@ static ScoreRows score_rows(const ScoreSaved& S, const void* saved) {
   return ScoreRows{reinterpret_cast<int*>(p + S.count), reinterpret_cast<int*>(p + S.row), reinterpret_cast<int64_t*>(p + S.token)};
 }
 struct ScoreScratch {
-  size_t dx, partial, total;
+  size_t dx, row_scale, partial, total;
 };
 static ScoreScratch score_scratch(long long N, long long H, long long V, bool want_dw, bool want_da) {
   ScoreScratch L;
   size_t o = 0, part = 0;
   L.dx = o;      o += up256((size_t)N * ((V + 7) & ~7LL) * 2);
+  L.row_scale = o; o += up256((size_t)N * 4);
   if (want_da) part = (size_t)plan_grad(N, H, V).splits * N * H * 4;  // its compact rows, in fp32 at most
   if (want_dw && plan_grad(V, H, N).splits > 1) part = std::max<size_t>(part, (size_t)plan_grad(V, H, N).splits * V * H * 4);
   L.partial = o; o += up256(part);
@@ -435,12 +443,13 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const auto* ab = reinterpret_cast<const __nv_bfloat16*>(sv + S.ab);
   const ScoreRows rows = score_rows(S, saved);
   auto* dx = reinterpret_cast<__nv_bfloat16*>(sc + L.dx);
+  auto* row_scale = reinterpret_cast<float*>(sc + L.row_scale);
   auto* part = reinterpret_cast<float*>(sc + L.partial);
   const int64_t shares = ((V + 7) / 8 + kDxShare - 1) / kDxShare;
   score_dx_kernel<<<(unsigned)(N * shares), kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
                                                                  reinterpret_cast<const float4*>(sv + S.score),
                                                                  reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, rows,
-                                                                 g_logprob, g_entropy, dx, S.ldV, (int)N, (int)V, S.groups,
+                                                                 g_logprob, g_entropy, dx, row_scale, S.ldV, (int)N, (int)V, S.groups,
                                                                  (uint32_t)shares);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
@@ -449,6 +458,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
     EpiParams ep{};
     ep.out_bf16 = plan.splits == 1 && da_dtype == HAWK_BF16;
     ep.count = rows.count;
+    ep.row_scale = row_scale;
     rc = plan.mh == 2 ? launch_gemm<EPI_OUT, 2, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, plan.splits, ep, status, st)
                       : launch_gemm<EPI_OUT, 1, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, plan.splits, ep, status, st);
     if (rc != HAWK_OK) return rc;

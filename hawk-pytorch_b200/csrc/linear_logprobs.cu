@@ -19,7 +19,8 @@
 //      probability, g_lp (1 - p) as -expm1; bf16 for the products, out of place: a second backward finds e as it was.  The token's
 //      element is most of its row, so the row is first scaled, by 2^-8 at most, to where that element is a bf16 number, and d act's
 //      row is scaled back as it leaves the product: its error is then that of its own rounding alone (1.7e-3 in norm where two
-//      roundings left 2.4e-3).  d W takes the rows as they are, which is the element's own rounding, as before.
+//      roundings left 2.4e-3).  d W takes the rows as they are, which is the element's own rounding; few rows it
+//      takes twice, as two bf16 numbers to each of fp32 (kTwiceRows).
 //   4. two GEMMs, d act = dx W and d W = dx^T act; d act's rows go back to their places.
 // Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16, all rows named:
 // 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.3 ms (1.36; dx 0.7 at 5.9 TB/s, the
@@ -31,12 +32,22 @@ namespace hawk {
 
 // What the forward finds out about its rows, on the device
 struct ScoreRows {
-  int* count;        // how many name a token: the compact rows 0 .. count - 1 below
+  int* count;        // how many name a token: the compact rows 0 .. count - 1 below; behind it the K rows of the d W product
   int* row;          // [N] compact row -> row
   int64_t* token;    // [N] compact row -> token (>= 0)
 };
-// compact rows up to here have to be zeros in the d W product, whose K blocks are of BK rows
-__device__ __forceinline__ int padded_count(int count, int N) { return min(N, (max(count, 1) + BK - 1) / BK * BK); }
+// The d W product reads whole K blocks of BK compact rows, zeros behind the last one.  Where few rows are named it reads each twice: as
+// many rows follow with what rounding d x to bf16 left, and act again.  (Sums of few terms do not average their roundings: d W
+// of 8 to 64 rows was 1.2 to 1.76 times as far off as a single rounding leaves it, and is 1.00 now; from 200 rows on 1.35 to 1.5, in
+// thousands 1.41 to 1.46.  The backward of 31 / 128 rows at H2048 V32000 takes 93 / 106 us instead of 88 / 96.)
+constexpr int kTwiceRows = 128;
+__host__ __device__ constexpr int64_t whole_blocks(int64_t rows) { return (rows + BK - 1) / BK * BK; }
+__device__ __forceinline__ int padded_count(int count) { return (int)whole_blocks(max(count, 1)); }
+__device__ __forceinline__ bool twice(int count) { return count <= kTwiceRows; }
+// rows that d x and the compact act have room for
+__host__ __device__ constexpr int64_t room_rows(int64_t N) {
+  return whole_blocks(N) > 2 * kTwiceRows ? whole_blocks(N) : 2 * whole_blocks(N) < 2 * kTwiceRows ? 2 * whole_blocks(N) : 2 * kTwiceRows;
+}
 
 // The first row_blocks blocks list `per` rows each (at most one to a thread): a block counts the named tokens before its own by
 // itself, so there is no second launch and no order between blocks.  That is N^2 / (2 per) tokens read from L2 in all: 75 MB at
@@ -105,7 +116,11 @@ score_prepare_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ a
       logprob[row] = entropy[row] = 0.f;
     }
   }
-  if (tid == 0 && first + own == N) *rows.count = before + total;
+  if (tid == 0 && first + own == N) {
+    const int n = before + total;
+    rows.count[0] = n;
+    rows.count[1] = twice(n) ? 2 * padded_count(n) : n;
+  }
   __syncthreads();
   const int vecs = H / 8, all = total * vecs;
 #pragma unroll 4
@@ -117,18 +132,23 @@ score_prepare_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ a
   }
 }
 
-// a warp to a compact row; `act` compact, and zeroed behind the last one as far as the d W product reads
+// a warp to a compact row; `act` compact, and completed as far as the d W product reads
 __global__ void __launch_bounds__(256)
 score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ correct, ScoreRows rows,
                     const __nv_bfloat16* __restrict__ weight, __nv_bfloat16* __restrict__ act, float* __restrict__ logprob,
-                    float* __restrict__ entropy, float2* __restrict__ stats, int N, int H, int V, int groups,
+                    float* __restrict__ entropy, float2* __restrict__ stats, int H, int V, int groups,
                     const int* __restrict__ status) {
   const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, count = *rows.count;
-  if (r >= count) {
-    if (r < padded_count(count, N))
-      for (int i = lane * 8; i < H; i += 256) *reinterpret_cast<uint4*>(act + (long long)r * H + i) = make_uint4(0u, 0u, 0u, 0u);
-    return;
+  if (r < padded_count(count)) {
+    uint4* again = twice(count) ? reinterpret_cast<uint4*>(act + (long long)(padded_count(count) + r) * H) : nullptr;
+    uint4* here = reinterpret_cast<uint4*>(act + (long long)r * H);
+    for (int i = lane; i < H / 8; i += 32) {
+      const uint4 v = r < count ? here[i] : make_uint4(0u, 0u, 0u, 0u);
+      if (r >= count) here[i] = v;
+      if (again) again[i] = v;
+    }
   }
+  if (r >= count) return;
   const float4* g = score + (long long)r * groups;
   const int64_t token = rows.token[r];
   float own = 0.f;
@@ -187,7 +207,7 @@ __global__ void __launch_bounds__(kDxThreads)
 score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
                 const float* __restrict__ logprob, const float* __restrict__ entropy, ScoreRows rows,
                 const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, float* __restrict__ row_scale,
-                long long ld, int N, int V, int groups, uint32_t shares) {
+                long long ld, int V, int groups, uint32_t shares) {
   const uint32_t r = blockIdx.x / shares;
   const int i0 = (int)(blockIdx.x - r * shares) * kDxShare + (int)threadIdx.x;
   const int nvec = (V + 7) / 8;  // ld is a multiple of 8; what lies behind V is never read
@@ -195,11 +215,15 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   const float4* g = score + (long long)r * groups;
   __nv_bfloat16* out = dx + r * ld;
   const int count = *rows.count;
+  __nv_bfloat16* rest = twice(count) ? out + padded_count(count) * ld : nullptr;
   if ((int)r >= count) {
-    if ((int)r >= padded_count(count, N)) return;
+    if ((int)r >= padded_count(count)) return;
 #pragma unroll
     for (int q = 0; q < kDxVectors; ++q)
-      if (i0 + q * kDxThreads < nvec) reinterpret_cast<uint4*>(out)[i0 + q * kDxThreads] = make_uint4(0u, 0u, 0u, 0u);
+      if (i0 + q * kDxThreads < nvec) {
+        reinterpret_cast<uint4*>(out)[i0 + q * kDxThreads] = make_uint4(0u, 0u, 0u, 0u);
+        if (rest) reinterpret_cast<uint4*>(rest)[i0 + q * kDxThreads] = make_uint4(0u, 0u, 0u, 0u);
+      }
     return;
   }
   uint4 raw[kDxVectors];
@@ -219,8 +243,8 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   const bool known = token < V;
   const float own = fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H)), own16 = __bfloat162float(__float2bfloat16(own));
   const bool scaled = fabsf(own) > 1e-30f && fabsf(own16) < 1e37f;
-  const float shrink = scaled ? own16 / own : 1.f;
-  if (blockIdx.x == r * shares && threadIdx.x == 0) row_scale[r] = scaled ? own / own16 : 1.f;
+  const float shrink = scaled ? own16 / own : 1.f, grow = scaled ? own / own16 : 1.f;
+  if (blockIdx.x == r * shares && threadIdx.x == 0) row_scale[r] = grow;
 #pragma unroll
   for (int q = 0; q < kDxVectors; ++q) {
     const int i = i0 + q * kDxThreads;
@@ -242,11 +266,18 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
       d[2 * k + 1] = c.y;
     }
     VecIO<__nv_bfloat16, 8>::store(out + (long long)i * 8, d);
+    if (rest) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[j] = fmaf(grow, d[j], -__bfloat162float(__float2bfloat16(d[j])));
+      VecIO<__nv_bfloat16, 8>::store(rest + (long long)i * 8, d);
+    }
   }
   // the token's own element anew, by the thread that wrote it
   const int64_t in_share = token / 8 - (i0 - (int)threadIdx.x);
-  if (known && in_share >= 0 && in_share < kDxShare && (int)threadIdx.x == (int)in_share % kDxThreads)
+  if (known && in_share >= 0 && in_share < kDxShare && (int)threadIdx.x == (int)in_share % kDxThreads) {
     out[token] = __float2bfloat16(own);
+    if (rest) rest[token] = __float2bfloat16(own - own16);
+  }
 }
 
 // d act from its compact rows: the sum over the splits of K, to the rows that they belong to, and zeros to the others.  A warp to 1024
@@ -303,7 +334,7 @@ static ScoreSaved score_saved(long long N, long long H, long long V, int w_dtype
   L.groups = (int)((V + EPI_COLS - 1) / EPI_COLS);
   size_t o = 0;
   L.wb = o;      o += w_dtype == HAWK_F32 ? up256((size_t)V * H * 2) : 0;
-  L.ab = o;      o += up256((size_t)N * H * 2);
+  L.ab = o;      o += up256((size_t)room_rows(N) * H * 2);
   L.count = o;   o += 256;
   L.row = o;     o += up256((size_t)N * 4);
   L.token = o;   o += up256((size_t)N * 8);
@@ -324,10 +355,11 @@ struct ScoreScratch {
 static ScoreScratch score_scratch(long long N, long long H, long long V, bool want_dw, bool want_da) {
   ScoreScratch L;
   size_t o = 0, part = 0;
-  L.dx = o;      o += up256((size_t)N * ((V + 7) & ~7LL) * 2);
+  L.dx = o;      o += up256((size_t)room_rows(N) * ((V + 7) & ~7LL) * 2);
   L.row_scale = o; o += up256((size_t)N * 4);
   if (want_da) part = (size_t)plan_grad(N, H, V).splits * N * H * 4;  // its compact rows, in fp32 at most
-  if (want_dw && plan_grad(V, H, N).splits > 1) part = std::max<size_t>(part, (size_t)plan_grad(V, H, N).splits * V * H * 4);
+  const long long splits = want_dw ? plan_grad(V, H, room_rows(N)).splits : 1;
+  if (splits > 1) part = std::max<size_t>(part, (size_t)splits * V * H * 4);
   L.partial = o; o += up256(part);
   L.total = o;
   return L;
@@ -363,7 +395,7 @@ extern "C" int hawk_linear_logprobs_kernels(int64_t N, int64_t H, int64_t V, int
   (void)a_dtype;
   if (N < 1 || H < 1 || V < 1) return 0;
   if (!want_dw && !want_da) return N > kCountedRows ? 4 : 3;
-  return 2 + (want_da ? 2 : 0) + (want_dw ? (plan_grad(V, H, N).splits > 1 ? 2 : 1) : 0);
+  return 2 + (want_da ? 2 : 0) + (want_dw ? (plan_grad(V, H, room_rows(N)).splits > 1 ? 2 : 1) : 0);
 }
 
 extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const int64_t* tokens, float* logprob, float* entropy, void* saved,
@@ -414,8 +446,8 @@ extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const i
   else
     rc = launch_gemm<EPI_SCORE, 1, false, false>(ab, H, wb, H, nullptr, false, S.ldV, (int)N, (int)V, (int)H, 1, ep, status, st);
   if (rc != HAWK_OK) return rc;
-  score_reduce_kernel<<<(unsigned)((N + 7) / 8), 256, 0, st>>>(ep.score, correct, rows, wb, ab, logprob, entropy,
-                                                               reinterpret_cast<float2*>(sv + S.stats), (int)N, (int)H, (int)V, S.groups,
+  score_reduce_kernel<<<(unsigned)(whole_blocks(N) / 8), 256, 0, st>>>(ep.score, correct, rows, wb, ab, logprob, entropy,
+                                                               reinterpret_cast<float2*>(sv + S.stats), (int)H, (int)V, S.groups,
                                                                status);
   return launch_status();
 }
@@ -431,7 +463,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const ScoreSaved S = score_saved(N, H, V, w_dtype, true);
   const ScoreScratch L = score_scratch(N, H, V, dweight != nullptr, dact != nullptr);
   HAWK_REQUIRE(saved && saved_bytes >= S.total && scratch && scratch_bytes >= L.total, HAWK_ERR_WORKSPACE);
-  HAWK_REQUIRE(N * (H / 1024 + 1) < (1LL << 31) && N * (V / (8 * kDxShare) + 1) < (1LL << 31), HAWK_ERR_SHAPE);
+  HAWK_REQUIRE(N * (H / 1024 + 1) < (1LL << 31) && whole_blocks(N) * (V / (8 * kDxShare) + 1) < (1LL << 31), HAWK_ERR_SHAPE);
   HAWK_REQUIRE(aligned(saved, 256) && aligned(scratch, 256) && aligned(dweight, 16) && aligned(dact, 16) && aligned(weight, 16) &&
                    aligned(act, 16) && aligned(tokens, 8) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(g_logprob, 4) &&
                    aligned(g_entropy, 4),
@@ -446,10 +478,10 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   auto* row_scale = reinterpret_cast<float*>(sc + L.row_scale);
   auto* part = reinterpret_cast<float*>(sc + L.partial);
   const int64_t shares = ((V + 7) / 8 + kDxShare - 1) / kDxShare;
-  score_dx_kernel<<<(unsigned)(N * shares), kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
+  score_dx_kernel<<<(unsigned)(whole_blocks(N) * shares), kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
                                                                  reinterpret_cast<const float4*>(sv + S.score),
                                                                  reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, rows,
-                                                                 g_logprob, g_entropy, dx, row_scale, S.ldV, (int)N, (int)V, S.groups,
+                                                                 g_logprob, g_entropy, dx, row_scale, S.ldV, (int)V, S.groups,
                                                                  (uint32_t)shares);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
@@ -474,7 +506,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
     if (rc != HAWK_OK) return rc;
   }
   if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the compact rows of dx and act are the K index)
-    rc = grad_gemm<true, true>(dx, S.ldV, ab, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)N, rows.count, part, status, st);
+    rc = grad_gemm<true, true>(dx, S.ldV, ab, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)room_rows(N), rows.count + 1, part, status, st);
     if (rc != HAWK_OK) return rc;
   }
   ce_poison_on_abort_kernel<<<1, 1, 0, st>>>(status, dweight, dw_dtype == HAWK_BF16, dact, da_dtype == HAWK_BF16);

@@ -281,3 +281,16 @@ def test_activations_gradient_is_rounded_once(N, H, V, lift):
         a.requires_grad_()
         got, = torch.autograd.grad(linear_logprobs(w, a, t), a, (gl, ge))
         assert rel_l2(got, da) <= 1.1 * rel_l2(da.bfloat16(), da)
+
+
+@pytest.mark.parametrize("N", [1, 31, 64, 65, 128])
+def test_weights_gradient_of_few_rows_is_rounded_once(N):
+    """d x as two bf16 numbers holds 16 bits: the error in norm is that of rounding the 64-bit gradient, and 2^-16 / 2^-9 of it."""
+    from hawk_b200 import linear_logprobs
+    for seed in range(4):
+        w, a, t, gl, ge = _case(N, 96, 5802, seed)
+        _, _, dw, _ = _reference(w, a, t, gl, ge)
+        w.requires_grad_()
+        out = linear_logprobs(w, torch.cat((a, a)), torch.cat((t, torch.full_like(t, -1))))  # as many rows again left out
+        got, = torch.autograd.grad(out, w, (torch.cat((gl, gl)), torch.cat((ge, ge))))
+        assert rel_l2(got, dw) <= 1.05 * rel_l2(dw.bfloat16(), dw)

@@ -286,9 +286,14 @@ constexpr int kScatterVecs = 4;
 template <typename TC, typename TO>
 __global__ void __launch_bounds__(256)
 score_scatter_kernel(const TC* __restrict__ part, int splits, const int64_t* __restrict__ tokens, ScoreRows rows, TO* __restrict__ out,
-                     uint32_t units, uint32_t chunks, int N, int H) {
+                     uint32_t units, uint32_t chunks, int N, int H, const int* __restrict__ status, void* dw, int dw_bf16) {
   const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit >= units) return;
+  const bool failed = *status != 0;  // a GEMM gave up a wait: NaN in the rows of d act, and in d weight's first element
+  if (failed && dw && blockIdx.x == 0 && threadIdx.x == 0) {
+    if (dw_bf16) *static_cast<__nv_bfloat16*>(dw) = __float2bfloat16(__int_as_float(0x7fc00000));
+    else *static_cast<float*>(dw) = __int_as_float(0x7fc00000);
+  }
   const int r = (int)(unit / chunks), c0 = ((int)(unit - r * chunks) * 32 * kScatterVecs + (threadIdx.x & 31)) * 8;
   const bool mine = r < *rows.count;
   if (tokens[r] < 0) {
@@ -317,7 +322,13 @@ score_scatter_kernel(const TC* __restrict__ part, int splits, const int64_t* __r
   TO* to = out + (long long)rows.row[r] * H + c0;
 #pragma unroll
   for (int q = 0; q < kScatterVecs; ++q)
-    if (c0 + q * 256 < H) VecIO<TO, 8>::store(to + q * 256, v[q]);
+    if (c0 + q * 256 < H) {
+      if (failed) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[q][j] = __int_as_float(0x7fc00000);
+      }
+      VecIO<TO, 8>::store(to + q * 256, v[q]);
+    }
 }
 
 // ---- host --------------------------------------------------------------------------------------------------
@@ -388,14 +399,14 @@ extern "C" size_t hawk_linear_logprobs_scratch_bytes(int64_t N, int64_t H, int64
   return score_scratch(N, H, V, want_dw != 0, want_da != 0).total;
 }
 
-// the forward (want_dw = want_da = 0): the rows (counted before in long lists) and casts, the GEMM and the reduction; the backward: d x, a GEMM and the scatter or,
-// where K is split, the sum for each gradient, the look at the status word
+// the forward (want_dw = want_da = 0): the rows (counted before in long lists) and casts, the GEMM and the reduction; the backward:
+// d x, d weight's GEMM and, where K is split, the sum, d act's GEMM and the scatter, which looks at the status word, too
 extern "C" int hawk_linear_logprobs_kernels(int64_t N, int64_t H, int64_t V, int w_dtype, int a_dtype, int want_dw, int want_da) {
   (void)w_dtype;
   (void)a_dtype;
   if (N < 1 || H < 1 || V < 1) return 0;
   if (!want_dw && !want_da) return N > kCountedRows ? 4 : 3;
-  return 2 + (want_da ? 2 : 0) + (want_dw ? (plan_grad(V, H, room_rows(N)).splits > 1 ? 2 : 1) : 0);
+  return 1 + (want_da ? 2 : 1) + (want_dw ? (plan_grad(V, H, room_rows(N)).splits > 1 ? 2 : 1) : 0);
 }
 
 extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const int64_t* tokens, float* logprob, float* entropy, void* saved,
@@ -485,6 +496,10 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
                                                                  (uint32_t)shares);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
+  if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the compact rows of dx and act are the K index)
+    rc = grad_gemm<true, true>(dx, S.ldV, ab, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)room_rows(N), rows.count + 1, part, status, st);
+    if (rc != HAWK_OK) return rc;
+  }
   if (dact) {  // d act [N,H] = dx [N,V] . W [V,H]: A K-major, B MN-major (W's rows are the K index); compact rows
     const GradPlan plan = plan_grad(N, H, V);
     EpiParams ep{};
@@ -497,18 +512,14 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
     const int64_t chunks = (H + 256 * kScatterVecs - 1) / (256 * kScatterVecs), units = N * chunks;
     const unsigned blocks = (unsigned)((units + 7) / 8);
     const auto scatter = [&](const auto* from, int splits, auto* to) {
-      score_scatter_kernel<<<blocks, 256, 0, st>>>(from, splits, tokens, rows, to, (uint32_t)units, (uint32_t)chunks, (int)N, (int)H);
+      score_scatter_kernel<<<blocks, 256, 0, st>>>(from, splits, tokens, rows, to, (uint32_t)units, (uint32_t)chunks, (int)N, (int)H, status,
+                                                 dweight, dw_dtype == HAWK_BF16);
     };
     if (ep.out_bf16) scatter(reinterpret_cast<const __nv_bfloat16*>(part), 1, static_cast<__nv_bfloat16*>(dact));
     else if (da_dtype == HAWK_BF16) scatter(static_cast<const float*>(part), plan.splits, static_cast<__nv_bfloat16*>(dact));
     else scatter(static_cast<const float*>(part), plan.splits, static_cast<float*>(dact));
-    rc = launch_status();
-    if (rc != HAWK_OK) return rc;
+    return launch_status();
   }
-  if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the compact rows of dx and act are the K index)
-    rc = grad_gemm<true, true>(dx, S.ldV, ab, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)room_rows(N), rows.count + 1, part, status, st);
-    if (rc != HAWK_OK) return rc;
-  }
-  ce_poison_on_abort_kernel<<<1, 1, 0, st>>>(status, dweight, dw_dtype == HAWK_BF16, dact, da_dtype == HAWK_BF16);
+  ce_poison_on_abort_kernel<<<1, 1, 0, st>>>(status, dweight, dw_dtype == HAWK_BF16, nullptr, 0);
   return launch_status();
 }

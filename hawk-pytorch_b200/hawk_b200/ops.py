@@ -1880,9 +1880,9 @@ def linear_logprobs_bwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.T
     if N == 0:
         return dw.zero_(), da
     gl, ge = (None if g is None else g.float().contiguous() for g in (g_logprob, g_entropy))
-    ws = torch.empty(lib.hawk_linear_logprobs_scratch_bytes(N, H, V, _dt(act), int(want_dw), int(want_da)), dtype=torch.uint8, device=dev)
     with _on(act, "linear_logprobs_bwd",
              lambda: lib.hawk_linear_logprobs_kernels(N, H, V, _dt(weight), _dt(act), int(want_dw), int(want_da))):
+        ws = torch.empty(lib.hawk_linear_logprobs_scratch_bytes(N, H, V, _dt(act), int(want_dw), int(want_da)), dtype=torch.uint8, device=dev)
         _lib.check(lib.hawk_linear_logprobs_bwd(weight.data_ptr(), act.data_ptr(), tokens.data_ptr(), saved.data_ptr(), saved.numel(),
                                                 logprob.data_ptr(), entropy.data_ptr(), _ptr(gl), _ptr(ge), dw.data_ptr() if want_dw else None,
                                                 _dt(dw), da.data_ptr() if want_da else None, _dt(da), ws.data_ptr(), ws.numel(), N, H, V,

@@ -294,3 +294,29 @@ def test_weights_gradient_of_few_rows_is_rounded_once(N):
         out = linear_logprobs(w, torch.cat((a, a)), torch.cat((t, torch.full_like(t, -1))))  # as many rows again left out
         got, = torch.autograd.grad(out, w, (torch.cat((gl, gl)), torch.cat((ge, ge))))
         assert rel_l2(got, dw) <= 1.05 * rel_l2(dw.bfloat16(), dw)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("wanted", [(True, True), (True, False), (False, True)])
+def test_a_failure_shows_in_the_results(wanted, dtype):
+    """The status word as a kernel leaves it that gave up a wait (set here by hand): results and gradients are NaN, the check
+    raises once, and what follows is right again."""
+    from hawk_b200 import check_device_status, ops
+    w, a, t, gl, ge = _case(70, 64, 300, 17, dtype)
+    t[::3] = -1
+    lp, H, saved = ops.linear_logprobs_fwd(w, a, t, True)
+    good = ops.linear_logprobs_bwd(w, a, t, saved, lp, H, gl, ge, *wanted)
+    ops._status_word(w.device).fill_(1)
+    try:
+        bad = ops.linear_logprobs_fwd(w, a, t, True)
+        assert bool(bad[0][t >= 0].isnan().all()) and bool(bad[1][t >= 0].isnan().all())
+        dw, da = ops.linear_logprobs_bwd(w, a, t, saved, lp, H, gl, ge, *wanted)
+        assert not wanted[0] or bool(dw[0, 0].isnan())
+        assert not wanted[1] or (bool(da[t >= 0].isnan().all()) and bool((da[t < 0] == 0).all()))
+        with pytest.raises(RuntimeError, match="abandoned"):
+            check_device_status()
+    finally:
+        ops._status_word(w.device).zero_()
+    check_device_status()
+    again = ops.linear_logprobs_bwd(w, a, t, saved, lp, H, gl, ge, *wanted)
+    assert all(torch.equal(x, y) for x, y in zip(good, again))

@@ -50,6 +50,7 @@ struct EpiParams {
   // plans its tiles anew.  Null = all.  Rows of A behind it may hold anything; rows of K up to the next block's end hold zeros.
   const int* count;
   int count_is_k;
+  int part_rows;             // not 0, for a count of M: splits of K planned anew, too (CountedRows), in this many rows of partial sums
   // EPI_LOGITS
   float2* stats;             // [column groups of 128, M] (max, sum exp)
   float* correct;            // [M] logit at the label
@@ -162,11 +163,11 @@ __device__ __forceinline__ void box_put(unsigned char* box, int lane, int piece0
         make_uint4(p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]);
 }
 __device__ __forceinline__ void box_store(const CUtensorMap* map, const unsigned char* box, int lane, int col, int row,
-                                          int depth, const EpiParams& ep) {
+                                          int depth, const EpiParams& ep, int shift = 0) {
   fence_smem_to_tma();
   __syncwarp();
   if (lane == 0) {
-    if (col < ep.Nc && row < ep.M) tma_store_3d(map, box, col, row, depth);
+    if (col < ep.Nc && row < ep.M) tma_store_3d(map, box, col, row + shift, depth);
     bulk_commit();  // an empty group where nothing is stored: the group count stays in step
   }
 }
@@ -176,6 +177,20 @@ struct CountedSplits {
   int blocks, per, splits;
   __device__ __forceinline__ CountedSplits(int n, int most)
       : blocks(max(1, (n + BK - 1) / BK)), per((blocks + most - 1) / most), splits((blocks + per - 1) / per) {}
+};
+
+// The tiles of a count of M rows known on the device only: K in more splits than were planned for all rows where `pairs` of CTAs would be
+// left without a tile, in whole boxes of 32 rows of partial sums to a split
+struct CountedRows {
+  int m_tiles, per, splits, stride;
+  __device__ __forceinline__ CountedRows(int n, int tile_rows, int n_tiles, int kblocks, int planned, int part_rows, int pairs) {
+    m_tiles = (n + tile_rows - 1) / tile_rows;
+    stride = max(32, (n + 31) / 32 * 32);
+    const int most = min(min(kblocks, 32), max(1, part_rows / stride));
+    splits = min(max(planned, pairs / max(1, m_tiles * n_tiles)), most);
+    per = (kblocks + splits - 1) / splits;
+    splits = (kblocks + per - 1) / per;
+  }
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -189,6 +204,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GEMM_THREADS, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_c, int K, int m_tiles, int n_tiles, int splits, EpiParams ep,
                  int* status) {
+  int split_rows = 0;  // rows of partial sums to a split where the splits were planned here
   if (ep.count) {
     const int n = *ep.count;
     if (ep.count_is_k) {
@@ -196,6 +212,13 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
       K = c.blocks * BK;
       ep.k_per_split = c.per;
       splits = c.splits;
+    } else if (MODE == EPI_OUT && ep.part_rows) {
+      const CountedRows c(n, BM * MH, n_tiles, (K + BK - 1) / BK, splits, ep.part_rows, gridDim.x >> 1);
+      ep.M = n;
+      m_tiles = c.m_tiles;
+      ep.k_per_split = c.per;
+      splits = c.splits;
+      split_rows = c.stride;
     } else {
       ep.M = n;
       m_tiles = (n + BM * MH - 1) / (BM * MH);
@@ -418,7 +441,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         if (row_ok && col0 < ep.Nc) ep.stats[(long long)(col0 / EPI_COLS) * ep.M + row] = make_float2(run_m, run_s);
       } else {
-        const int split = tile / tiles;
+        const int in_split = tile / tiles, split = split_rows ? 0 : in_split, shift = in_split * split_rows;
         const float f = ep.row_scale && row_ok ? scale * __ldg(ep.row_scale + row) : scale;
         auto chunk = [&](int c) -> const uint32_t(&)[32] {  // waits for chunk c, requests the next one
           tmem_ld_wait();
@@ -436,7 +459,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             unsigned char* box = boxes + ((c >> 1) % Cfg::NBOX) * BOX_BYTES;
             if ((c & 1) == 0) box_reuse<Cfg::NBOX>(lane);
             box_put(box, lane, (c & 1) * 4, packed);
-            if (c & 1) box_store(&map_c, box, lane, col0 + (c >> 1) * 64, row0, split, ep);
+            if (c & 1) box_store(&map_c, box, lane, col0 + (c >> 1) * 64, row0, split, ep, shift);
           }
         } else {
 #pragma unroll
@@ -451,7 +474,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
               for (int j = 0; j < 16; ++j) scaled[j] = __float_as_uint(__uint_as_float(w[16 * q + j]) * f);
               box_put(box, lane, q * 4, scaled);
             }
-            box_store(&map_c, box, lane, col0 + c * 32, row0, split, ep);
+            box_store(&map_c, box, lane, col0 + c * 32, row0, split, ep, shift);
           }
         }
       }
@@ -519,7 +542,9 @@ static int launch_gemm(const __nv_bfloat16* A, long long lda, const __nv_bfloat1
   const bool okb = B_MN ? make_map_bf16(&mb, B, K, Nc, ldb, 64) : make_map_bf16(&mb, B, Nc, K, ldb, 128);
   if (!oka || !okb) return HAWK_ERR_DEVICE;
   if (!C) mc = ma;  // nothing is stored through it
-  else if (!make_map_store(&mc, C, c_f32, Nc, M, splits, ldc, (long long)M * ldc)) return HAWK_ERR_DEVICE;
+  else if (ep.part_rows ? !make_map_store(&mc, C, c_f32, Nc, ep.part_rows, 1, ldc, (long long)ep.part_rows * ldc)
+                        : !make_map_store(&mc, C, c_f32, Nc, M, splits, ldc, (long long)M * ldc))
+    return HAWK_ERR_DEVICE;
   auto kern = gemm_bf16_kernel<MODE, MH, A_MN, B_MN>;
   constexpr int GEMM_SMEM = GemmCfg<MH>::SMEM;
   // per call: the attribute belongs to the current device's copy of the kernel
@@ -532,7 +557,7 @@ static int launch_gemm(const __nv_bfloat16* A, long long lda, const __nv_bfloat1
   ep.Nc = Nc;
   ep.k_per_split = (kblocks + splits - 1) / splits;
   const long long work = (long long)m_tiles * n_tiles * splits;
-  const int pairs = (int)std::min<long long>(work, sm_count() / 2);
+  const int pairs = ep.part_rows ? sm_count() / 2 : (int)std::min<long long>(work, sm_count() / 2);
   kern<<<2 * pairs, GEMM_THREADS, GEMM_SMEM, st>>>(ma, mb, mc, K, m_tiles, n_tiles, splits, ep, status);
   return launch_status();
 }

@@ -280,13 +280,15 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   }
 }
 
-// d act from its compact rows: the sum over the splits of K, to the rows that they belong to, and zeros to the others.  A warp to 1024
-// columns of a row, 4 vectors of 8 to a lane.  N32760 H2048 in bf16 48 us (a thread to a vector, which divides 64-bit numbers: 68)
-constexpr int kScatterVecs = 4;
-template <typename TC, typename TO>
+// d act from its compact rows: the sum over the splits of K, to the rows that they belong to, and zeros to the others.  A warp to 256
+// columns of a row, a vector of 8 to a lane, or to 1024 where there is nothing to add up.  N32760 H2048 in bf16 48 us (a thread to a vector, which divides 64-bit numbers: 68)
+struct ScatterPlan {  // what the GEMM knew when it planned its splits (part_rows 0: one, no partial sums)
+  int tile_rows, n_tiles, kblocks, planned, part_rows, pairs;
+};
+template <typename TC, typename TO, int kVecs>
 __global__ void __launch_bounds__(256)
-score_scatter_kernel(const TC* __restrict__ part, int splits, const int64_t* __restrict__ tokens, ScoreRows rows, TO* __restrict__ out,
-                     uint32_t units, uint32_t chunks, int N, int H, const int* __restrict__ status, void* dw, int dw_bf16) {
+score_scatter_kernel(const TC* __restrict__ part, ScatterPlan plan, const int64_t* __restrict__ tokens, ScoreRows rows, TO* __restrict__ out,
+                     uint32_t units, uint32_t chunks, int H, const int* __restrict__ status, void* dw, int dw_bf16) {
   const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (unit >= units) return;
   const bool failed = *status != 0;  // a GEMM gave up a wait: NaN in the rows of d act, and in d weight's first element
@@ -294,24 +296,32 @@ score_scatter_kernel(const TC* __restrict__ part, int splits, const int64_t* __r
     if (dw_bf16) *static_cast<__nv_bfloat16*>(dw) = __float2bfloat16(__int_as_float(0x7fc00000));
     else *static_cast<float*>(dw) = __int_as_float(0x7fc00000);
   }
-  const int r = (int)(unit / chunks), c0 = ((int)(unit - r * chunks) * 32 * kScatterVecs + (threadIdx.x & 31)) * 8;
+  const int r = (int)(unit / chunks), c0 = ((int)(unit - r * chunks) * 32 * kVecs + (threadIdx.x & 31)) * 8;
   const bool mine = r < *rows.count;
   if (tokens[r] < 0) {
     const float zero[8] = {};
 #pragma unroll
-    for (int q = 0; q < kScatterVecs; ++q)
+    for (int q = 0; q < kVecs; ++q)
       if (c0 + q * 256 < H) VecIO<TO, 8>::store(out + (long long)r * H + c0 + q * 256, zero);
   }
   if (!mine) return;
-  float v[kScatterVecs][8];
+  float v[kVecs][8];
   const TC* in = part + (long long)r * H + c0;
 #pragma unroll
-  for (int q = 0; q < kScatterVecs; ++q)
+  for (int q = 0; q < kVecs; ++q)
     if (c0 + q * 256 < H) VecIO<TC, 8>::load(in + q * 256, v[q]);
+  int splits = 1;
+  long long stride = 0;
+  if (plan.part_rows) {
+    const CountedRows c(*rows.count, plan.tile_rows, plan.n_tiles, plan.kblocks, plan.planned, plan.part_rows, plan.pairs);
+    splits = c.splits;
+    stride = (long long)c.stride * H;
+  }
+#pragma unroll 4
   for (int s = 1; s < splits; ++s) {
-    in += (long long)N * H;
+    in += stride;
 #pragma unroll
-    for (int q = 0; q < kScatterVecs; ++q)
+    for (int q = 0; q < kVecs; ++q)
       if (c0 + q * 256 < H) {
         float u[8];
         VecIO<TC, 8>::load(in + q * 256, u);
@@ -321,7 +331,7 @@ score_scatter_kernel(const TC* __restrict__ part, int splits, const int64_t* __r
   }
   TO* to = out + (long long)rows.row[r] * H + c0;
 #pragma unroll
-  for (int q = 0; q < kScatterVecs; ++q)
+  for (int q = 0; q < kVecs; ++q)
     if (c0 + q * 256 < H) {
       if (failed) {
 #pragma unroll
@@ -363,12 +373,20 @@ static ScoreRows score_rows(const ScoreSaved& S, const void* saved) {
 struct ScoreScratch {
   size_t dx, row_scale, partial, total;
 };
+// d act of up to this many rows leaves partial sums in fp32 over splits of K that its kernel plans for the rows that are named (3108 rows
+// of 2048, V32000, nine of ten left out: backward 386 -> 143 us, half 519 -> 393); of more rows even a tenth fills the GPU, and their product leaves what it is
+// asked for
+constexpr int64_t kPlannedRows = 8192;
+static int da_part_rows(int64_t N, const GradPlan& plan) {  // 0: no partial sums
+  const int64_t rows = plan.splits * ((N + 31) / 32 * 32);
+  return (N <= kPlannedRows || plan.splits > 1) && rows < (1LL << 31) ? (int)rows : 0;
+}
 static ScoreScratch score_scratch(long long N, long long H, long long V, bool want_dw, bool want_da) {
   ScoreScratch L;
   size_t o = 0, part = 0;
   L.dx = o;      o += up256((size_t)room_rows(N) * ((V + 7) & ~7LL) * 2);
   L.row_scale = o; o += up256((size_t)N * 4);
-  if (want_da) part = (size_t)plan_grad(N, H, V).splits * N * H * 4;  // its compact rows, in fp32 at most
+  if (want_da) part = (size_t)std::max<int64_t>(N, da_part_rows(N, plan_grad(N, H, V))) * H * 4;  // its compact rows, in fp32 at most
   const long long splits = want_dw ? plan_grad(V, H, room_rows(N)).splits : 1;
   if (splits > 1) part = std::max<size_t>(part, (size_t)splits * V * H * 4);
   L.partial = o; o += up256(part);
@@ -474,7 +492,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const ScoreSaved S = score_saved(N, H, V, w_dtype, true);
   const ScoreScratch L = score_scratch(N, H, V, dweight != nullptr, dact != nullptr);
   HAWK_REQUIRE(saved && saved_bytes >= S.total && scratch && scratch_bytes >= L.total, HAWK_ERR_WORKSPACE);
-  HAWK_REQUIRE(N * (H / 1024 + 1) < (1LL << 31) && whole_blocks(N) * (V / (8 * kDxShare) + 1) < (1LL << 31), HAWK_ERR_SHAPE);
+  HAWK_REQUIRE(N * (H / 256 + 1) < (1LL << 31) && whole_blocks(N) * (V / (8 * kDxShare) + 1) < (1LL << 31), HAWK_ERR_SHAPE);
   HAWK_REQUIRE(aligned(saved, 256) && aligned(scratch, 256) && aligned(dweight, 16) && aligned(dact, 16) && aligned(weight, 16) &&
                    aligned(act, 16) && aligned(tokens, 8) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(g_logprob, 4) &&
                    aligned(g_entropy, 4),
@@ -503,21 +521,26 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   if (dact) {  // d act [N,H] = dx [N,V] . W [V,H]: A K-major, B MN-major (W's rows are the K index); compact rows
     const GradPlan plan = plan_grad(N, H, V);
     EpiParams ep{};
-    ep.out_bf16 = plan.splits == 1 && da_dtype == HAWK_BF16;
+    ep.part_rows = da_part_rows(N, plan);
+    const int splits = ep.part_rows ? plan.splits : 1;
+    ep.out_bf16 = !ep.part_rows && da_dtype == HAWK_BF16;
     ep.count = rows.count;
     ep.row_scale = row_scale;
-    rc = plan.mh == 2 ? launch_gemm<EPI_OUT, 2, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, plan.splits, ep, status, st)
-                      : launch_gemm<EPI_OUT, 1, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, plan.splits, ep, status, st);
+    rc = plan.mh == 2 ? launch_gemm<EPI_OUT, 2, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, splits, ep, status, st)
+                      : launch_gemm<EPI_OUT, 1, false, true>(dx, S.ldV, wb, H, part, !ep.out_bf16, H, (int)N, (int)H, (int)V, splits, ep, status, st);
     if (rc != HAWK_OK) return rc;
-    const int64_t chunks = (H + 256 * kScatterVecs - 1) / (256 * kScatterVecs), units = N * chunks;
+    const int cols = ep.part_rows ? 256 : 1024;
+    const int64_t chunks = (H + cols - 1) / cols, units = N * chunks;
     const unsigned blocks = (unsigned)((units + 7) / 8);
-    const auto scatter = [&](const auto* from, int splits, auto* to) {
-      score_scatter_kernel<<<blocks, 256, 0, st>>>(from, splits, tokens, rows, to, (uint32_t)units, (uint32_t)chunks, (int)N, (int)H, status,
-                                                 dweight, dw_dtype == HAWK_BF16);
+    const ScatterPlan how{BM * plan.mh, (int)((H + BN - 1) / BN), (int)((V + BK - 1) / BK), plan.splits, ep.part_rows, sm_count() / 2};
+    const auto scatter = [&](auto kern, auto* from, auto* to) {
+      kern<<<blocks, 256, 0, st>>>(from, how, tokens, rows, to, (uint32_t)units, (uint32_t)chunks, (int)H, status, dweight, dw_dtype == HAWK_BF16);
     };
-    if (ep.out_bf16) scatter(reinterpret_cast<const __nv_bfloat16*>(part), 1, static_cast<__nv_bfloat16*>(dact));
-    else if (da_dtype == HAWK_BF16) scatter(static_cast<const float*>(part), plan.splits, static_cast<__nv_bfloat16*>(dact));
-    else scatter(static_cast<const float*>(part), plan.splits, static_cast<float*>(dact));
+    using bf16 = __nv_bfloat16;
+    if (ep.out_bf16) scatter(score_scatter_kernel<bf16, bf16, 4>, reinterpret_cast<bf16*>(part), static_cast<bf16*>(dact));
+    else if (da_dtype == HAWK_BF16) scatter(score_scatter_kernel<float, bf16, 1>, part, static_cast<bf16*>(dact));
+    else if (ep.part_rows) scatter(score_scatter_kernel<float, float, 1>, part, static_cast<float*>(dact));
+    else scatter(score_scatter_kernel<float, float, 4>, part, static_cast<float*>(dact));
     return launch_status();
   }
   ce_poison_on_abort_kernel<<<1, 1, 0, st>>>(status, dweight, dw_dtype == HAWK_BF16, nullptr, 0);

@@ -320,3 +320,12 @@ def test_a_failure_shows_in_the_results(wanted, dtype):
     check_device_status()
     again = ops.linear_logprobs_bwd(w, a, t, saved, lp, H, gl, ge, *wanted)
     assert all(torch.equal(x, y) for x, y in zip(good, again))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("N", [8192, 8193])
+def test_activations_gradient_of_many_rows(N, dtype):
+    """Both sides of where its splits are planned on the device, few and many of the rows named, fp32 and bf16 results."""
+    w, a, t, gl, ge = _case(N, 64, 1000, 18, dtype)
+    for every in (1, 2, 40):
+        _check(w, a, torch.where(torch.arange(N, device="cuda") % every == 0, t, -1), gl, ge)

@@ -16,7 +16,8 @@
 // Backward, from e and the groups' maxima (2 N V bytes kept instead of a third GEMM: forming the logits again takes 2 N H V
 // flops, 3.1 ms at N32760 H2048 V32000 where writing and reading e takes 1):
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
-//      probability, g_lp (1 - p) as -expm1; bf16 for the products, out of place: a second backward finds e as it was.  The token's
+//      probability, g_lp (1 - p) as -expm1 (log p_j of the others is that of the rounded e_j, 2^-12 off: where the two terms of a
+//      small vocabulary nearly cancel, that much of g_H p_j is left); bf16 for the products, out of place: a second backward finds e as it was.  The token's
 //      element is most of its row, so the row is first scaled, by 2^-8 at most, to where that element is a bf16 number, and d act's
 //      row is scaled back as it leaves the product: its error is then that of its own rounding alone (1.7e-3 in norm where two
 //      roundings left 2.4e-3).  d W takes the rows as they are, which is the element's own rounding; few rows it

@@ -117,10 +117,12 @@ class _on:
 # operators
 # ---------------------------------------------------------------------------------------------
 def _probes():
-    """What _plain_call asks of torch under private names; None where this torch lacks one of them."""
+    """What _plain_call, _has_tangent and _embed_backward ask of torch under private names; None where this torch lacks one of them."""
     C = torch._C
     try:
         torch.autograd.forward_ad._current_level, torch.autograd.profiler._is_profiler_enabled
+        C._functorch.is_batchedtensor, C._functorch.is_functorch_wrapped_tensor, C._functorch.get_unwrapped
+        C._functorch.is_legacy_batchedtensor
         return (C._len_torch_dispatch_stack, C._len_torch_function_stack, C._functorch.peek_interpreter_stack, C._get_tracing_state)
     except AttributeError:
         return None
@@ -153,6 +155,21 @@ def _plain_call(args) -> Optional[bool]:
     return grad and torch.is_grad_enabled()
 
 
+def _transformed() -> bool:
+    """Whether a functorch transform or a forward-mode level is active."""
+    return _PROBES is not None and (_PROBES[2]() is not None or torch.autograd.forward_ad._current_level >= 0)
+
+
+def _has_tangent(t) -> bool:
+    """Whether a tensor carries a tangent, at any of the levels that transforms have wrapped around it."""
+    functorch = torch._C._functorch
+    while isinstance(t, torch.Tensor):
+        if not functorch.is_batchedtensor(t) and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            return True
+        t = functorch.get_unwrapped(t) if functorch.is_functorch_wrapped_tensor(t) else None
+    return False
+
+
 class _Operator(torch.library.CustomOpDef):
     """A torch.library operator whose ordinary eager calls run its Python function directly, with autograd through one
     torch.autograd.Function.  The dispatcher's way through a Python operator costs 40 to 60 us of host time per call, more
@@ -161,11 +178,12 @@ class _Operator(torch.library.CustomOpDef):
     so does every call once something was registered that the direct way would pass by."""
 
     @classmethod
-    def make(cls, name, mutates_args, fn):
+    def make(cls, name, mutates_args, reverse_only, fn):
         self = torch.library.custom_op(name, mutates_args=mutates_args)(fn)
         self.__class__ = cls
         parameters = inspect.signature(fn).parameters
         names = list(parameters)
+        self.reverse_only = reverse_only
         self.direct, self.direct_fn, self.direct_autograd, self.direct_nargs = True, fn, None, len(names)
         self.direct_defaults = tuple(p.default for p in parameters.values() if p.default is not p.empty)
         self.direct_mutated = [names.index(m) for m in mutates_args]
@@ -202,6 +220,9 @@ class _Operator(torch.library.CustomOpDef):
                 return out
             if record and self.direct_autograd is not None:
                 return self.direct_autograd.apply(*args)
+        if (self.reverse_only and not torch.compiler.is_compiling() and _transformed()
+                and any(map(_has_tangent, (*args, *kwargs.values())))):  # the dispatcher would drop the tangents
+            raise NotImplementedError(f"hawk_b200: {self.__name__} has no forward-mode derivative")
         return super().__call__(*args, **kwargs)
 
 
@@ -218,8 +239,9 @@ for _name in ("register_kernel", "register_autocast", "register_torch_dispatch",
         setattr(_Operator, _name, _through_dispatcher(_name))
 
 
-def _operator(name, mutates_args):
-    return lambda fn: _Operator.make(name, mutates_args, fn)
+def _operator(name, mutates_args, reverse_only=False):
+    """reverse_only: a tangent is refused."""
+    return lambda fn: _Operator.make(name, mutates_args, reverse_only, fn)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -1742,7 +1764,7 @@ def _logit_rows(t: torch.Tensor):
     return t, ld
 
 
-@_operator("hawk_b200::token_logprobs_fwd", mutates_args=())
+@_operator("hawk_b200::token_logprobs_fwd", mutates_args=(), reverse_only=True)
 def token_logprobs_fwd(logits: torch.Tensor, tokens: torch.Tensor, top: int
                        ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(logprob, entropy, top_logprobs, top_ids, stats) of token_logprobs; stats [.., 2] is what the backward needs."""
@@ -1771,7 +1793,7 @@ def _(logits, tokens, top):
     return f(), f(), f(top), f(top, dtype=torch.int64), f(2)
 
 
-@_operator("hawk_b200::token_logprobs_bwd", mutates_args=())
+@_operator("hawk_b200::token_logprobs_bwd", mutates_args=(), reverse_only=True)
 def token_logprobs_bwd(logits: torch.Tensor, tokens: torch.Tensor, stats: torch.Tensor, logprob: torch.Tensor, entropy: torch.Tensor,
                        g_logprob: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor]) -> torch.Tensor:
     """The gradient of token_logprobs' logits."""
@@ -1827,7 +1849,7 @@ def token_logprobs(logits, tokens, top: int = 0):
     probabilities, by falling logit and, among equals, rising id.  One read of the logits, fp32 arithmetic; logprob and entropy are
     differentiable, the alternatives are not.  A negative token leaves its row out: 0 and 0, no gradient, alternatives -inf and -1,
     whatever the row holds.  A token >= V gives NaN.  Logits of -inf are tokens that cannot come; a row of nothing else has log
-    probability -inf, entropy 0 and no gradient."""
+    probability -inf, entropy 0 and no gradient.  A tangent is refused."""
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"hawk_b200: logits of shape {tuple(logits.shape)}")
     if not 0 <= top <= min(32, logits.shape[-1]):
@@ -1836,7 +1858,7 @@ def token_logprobs(logits, tokens, top: int = 0):
 
 
 # the same from activations and the head's weight, without logits in memory
-@_operator("hawk_b200::linear_logprobs_fwd", mutates_args=())
+@_operator("hawk_b200::linear_logprobs_fwd", mutates_args=(), reverse_only=True)
 def linear_logprobs_fwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.Tensor, want_grad: bool
                         ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(logprob, entropy, saved) of linear_logprobs; with want_grad `saved` holds what linear_logprobs_bwd needs."""
@@ -1866,7 +1888,7 @@ def _(weight, act, tokens, want_grad):
     return (*(act.new_empty(tokens.shape, dtype=torch.float32) for _ in range(2)), act.new_empty(n, dtype=torch.uint8))
 
 
-@_operator("hawk_b200::linear_logprobs_bwd", mutates_args=())
+@_operator("hawk_b200::linear_logprobs_bwd", mutates_args=(), reverse_only=True)
 def linear_logprobs_bwd(weight: torch.Tensor, act: torch.Tensor, tokens: torch.Tensor, saved: torch.Tensor, logprob: torch.Tensor,
                         entropy: torch.Tensor, g_logprob: Optional[torch.Tensor], g_entropy: Optional[torch.Tensor], want_dw: bool,
                         want_da: bool) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -1921,7 +1943,7 @@ def linear_logprobs(weight, act, tokens):
     mean loss: bf16 tensor-core products (operands in fp32 are rounded, as there), but the logits stay unrounded fp32 sums and are
     never in memory; a forward that waits for its backward holds N * V 16-bit values.  Negative tokens and those >= V as in
     token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold, and takes no time in the
-    products (the rows that name a token are listed on the device)."""
+    products (the rows that name a token are listed on the device).  A tangent is refused."""
     if weight.dim() != 2 or act.dim() < 1 or act.shape[-1] != weight.shape[1]:
         raise ValueError(f"hawk_b200: activations of shape {tuple(act.shape)} with a weight of shape {tuple(weight.shape)}")
     want = torch.is_grad_enabled() and (weight.requires_grad or act.requires_grad)
@@ -1931,7 +1953,7 @@ def linear_logprobs(weight, act, tokens):
 # ---------------------------------------------------------------------------------------------
 # embedding
 # ---------------------------------------------------------------------------------------------
-@_operator("hawk_b200::embedding_fwd", mutates_args=())
+@_operator("hawk_b200::embedding_fwd", mutates_args=(), reverse_only=True)
 def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: int = -1) -> torch.Tensor:
     """scale * weight[ids], in weight's dtype; ids int64 of any shape."""
     _same_device(weight, ids)
@@ -1951,7 +1973,7 @@ def _(ids, weight, scale=1.0, padding_idx=-1):
     return weight.new_empty((*ids.shape, weight.shape[1]))
 
 
-@_operator("hawk_b200::embedding_bwd", mutates_args=())
+@_operator("hawk_b200::embedding_bwd", mutates_args=(), reverse_only=True)
 def embedding_bwd(ids: torch.Tensor, dout: torch.Tensor, V: int, scale: float, padding_idx: int) -> torch.Tensor:
     """The gradient of embedding_fwd's weight, [V, H] in dout's dtype."""
     _same_device(dout, ids)
@@ -1981,7 +2003,10 @@ def _embed_setup(ctx, inputs, output):
 
 
 def _embed_backward(ctx, dout):
-    return None, embedding_bwd(ctx.saved_tensors[0], dout, ctx.V, ctx.scale, ctx.padding_idx), None, None
+    bwd = embedding_bwd
+    if _PROBES is not None and torch._C._functorch.is_legacy_batchedtensor(dout):  # is_grads_batched: the dispatcher takes such a gradient apart
+        bwd = super(_Operator, bwd).__call__
+    return None, bwd(ctx.saved_tensors[0], dout, ctx.V, ctx.scale, ctx.padding_idx), None, None
 
 
 embedding_fwd.register_autograd(_embed_backward, setup_context=_embed_setup)
@@ -2004,7 +2029,8 @@ embedding_bwd.register_autograd(_embed_bwd_backward, setup_context=_embed_bwd_se
 def embedding(ids, weight, scale: float = 1.0, padding_idx: Optional[int] = None):
     """scale * weight[ids] (weight [V,H] fp32 or bf16, ids of any shape and integer type), in weight's dtype.  The gradient of
     `weight` is dense, summed in fp32 in the order of the positions (the same bits on every run) and rounded once; the row
-    `padding_idx` gets none.  An id outside [0, V) gives a row of NaN and no gradient."""
+    `padding_idx` gets none.  An id outside [0, V) gives a row of NaN and no gradient.  A tangent is refused (`model.Embedding` takes
+    nn.Embedding's way under forward mode)."""
     if weight.dim() != 2:
         raise ValueError(f"hawk_b200: an embedding table has two dimensions, not {weight.dim()}")
     if ids.dtype != torch.int64:

@@ -133,3 +133,33 @@ def test_linear_logprobs_refuses_cpu_tensors():
     from hawk_b200 import linear_logprobs
     with pytest.raises(RuntimeError, match="CUDA"):
         linear_logprobs(torch.zeros(9, 8), torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64))
+
+
+# what may ask for a forward-mode derivative, each the derivative of f at x in the direction t
+def _dual(f, x, t):
+    with torch.autograd.forward_ad.dual_level():
+        return torch.autograd.forward_ad.unpack_dual(f(torch.autograd.forward_ad.make_dual(x, t))).tangent
+
+
+FORWARD_MODE = [_dual, lambda f, x, t: torch.func.jvp(f, (x,), (t,))[1], lambda f, x, t: torch.func.jacfwd(f)(x),
+                lambda f, x, t: torch.func.jvp(torch.func.vmap(f), (x,), (t,)), lambda f, x, t: torch.func.jvp(lambda a: f(x=a), (x,), (t,)),
+                lambda f, x, t: torch.func.jvp(lambda a: torch.func.jvp(f, (a,), (t,))[1], (x,), (t,))]
+
+
+@pytest.mark.parametrize("way", range(len(FORWARD_MODE)))
+def test_operators_without_a_forward_derivative_refuse_tangents(way):
+    """Operators of the form of the embedding and the log probabilities: the dispatcher would answer with a tangent of zeros."""
+    from hawk_b200 import ops
+
+    @ops._operator(f"hawk_b200_test::reverse_only_{way}", mutates_args=(), reverse_only=True)
+    def op(x: torch.Tensor) -> torch.Tensor:
+        return 2 * x
+    op.register_autograd(lambda ctx, g: 2 * g, setup_context=lambda ctx, inputs, output: None)
+    x, t = torch.ones(3, 2), torch.ones(3, 2)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        FORWARD_MODE[way](op, x, t)
+    assert torch.equal(torch.func.vmap(op)(x), 2 * x)  # other transforms are answered as before
+    with torch.autograd.forward_ad.dual_level():
+        assert torch.equal(op(x), 2 * x)  # no tangent
+    assert all(o.reverse_only for o in (ops.embedding_fwd, ops.embedding_bwd, ops.token_logprobs_fwd, ops.token_logprobs_bwd,
+                                        ops.linear_logprobs_fwd, ops.linear_logprobs_bwd))

@@ -220,3 +220,42 @@ def test_few_tokens_outside_the_table():
     want = torch.zeros(10, 12, device="cuda")
     want[3], want[9] = 6.0, 4.0
     assert torch.equal(dw, want)
+
+
+def test_module_under_transforms():
+    """Forward mode and torch.func see nn.Embedding's own code; the operator itself refuses tangents."""
+    import hawk_b200.model as M
+    from hawk_b200 import embedding, linear_logprobs, token_logprobs
+    from torch.autograd import forward_ad
+    from torch.func import functional_call, grad, jacfwd, jacrev, jvp, vmap
+    torch.manual_seed(0)
+    e = M.Embedding(6, 4, scale=2.0, padding_idx=3).cuda()
+    ids = torch.tensor([[1, 5, 3], [0, 1, 1]], device="cuda")
+    w, t = e.weight.detach().clone(), torch.randn(6, 4, device="cuda")
+    f = lambda w: functional_call(e, {"weight": w}, (ids,))  # noqa: E731
+    out, tangent = jvp(f, (w,), (t,))
+    assert torch.equal(out, 2 * w[ids]) and torch.equal(tangent, 2 * t[ids])
+    with forward_ad.dual_level():
+        assert torch.equal(forward_ad.unpack_dual(f(forward_ad.make_dual(w, t))).tangent, 2 * t[ids])
+    counts = torch.tensor([1.0, 3.0, 0.0, 0.0, 0.0, 1.0], device="cuda")  # padding has no gradient
+    assert torch.equal(grad(lambda w: f(w).sum())(w), 2 * counts[:, None].expand(6, 4))
+    jac = torch.zeros(2, 3, 4, 6, 4, device="cuda")
+    for i in range(2):
+        for k in range(3):
+            jac[i, k, range(4), ids[i, k], range(4)] = 2.0
+    rev = jac.clone()
+    rev[0, 2] = 0.0
+    assert torch.equal(jacfwd(f)(w), jac) and torch.equal(jacrev(f)(w), rev)
+    both = torch.stack([w, t])
+    assert torch.equal(vmap(f)(both), 2 * both[:, ids])
+    out = e(ids)  # a batch of upstream gradients for a forward without transforms
+    many, = torch.autograd.grad(out, e.weight, torch.stack([torch.ones_like(out), 3 * torch.ones_like(out)]), is_grads_batched=True)
+    assert torch.equal(many, torch.stack([k * 2 * counts[:, None].expand(6, 4) for k in (1, 3)]))
+    act, head, tokens = torch.randn(3, 8, device="cuda"), torch.randn(5, 8, device="cuda"), torch.zeros(3, dtype=torch.int64, device="cuda")
+    for f, x in ((lambda w: embedding(ids, w), w), (lambda a: linear_logprobs(head, a, tokens)[0], act),
+                 (lambda x: token_logprobs(x, tokens)[1], act)):
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            jvp(f, (x,), (torch.ones_like(x),))
+    out = e(ids)
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.autograd.grad(out, e.weight, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))

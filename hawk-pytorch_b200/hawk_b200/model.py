@@ -207,8 +207,9 @@ def drop_bf16_copies(module: nn.Module) -> None:
 class Embedding(nn.Embedding):
     """nn.Embedding (same parameter name and state-dict key, hawk/hawk.py:262) on `ops.embedding` for CUDA tables in fp32 or bf16:
     `scale` multiplies the rows in the same pass (1, the reference's model, leaves them as they are; models of this family also
-    use sqrt(width)), and the gradient is summed by token in a fixed order.  `max_norm`, `scale_grad_by_freq` and `sparse`, and
-    calls under torch.func's transforms or forward-mode differentiation, are nn.Embedding's own code."""
+    use sqrt(width)), and the gradient is summed by token in a fixed order.  `max_norm`, `scale_grad_by_freq` and `sparse`,
+    tables and ids of a tensor subclass (a sharded table), and calls under torch.func's transforms or forward-mode differentiation
+    are nn.Embedding's own code."""
 
     def __init__(self, *args, scale: float = 1.0, **kwargs):
         super().__init__(*args, **kwargs)
@@ -217,7 +218,8 @@ class Embedding(nn.Embedding):
     def forward(self, ids):
         w = self.weight
         if (not w.is_cuda or w.dtype not in (torch.float32, torch.bfloat16) or self.max_norm is not None or self.scale_grad_by_freq
-                or self.sparse or (not torch.compiler.is_compiling() and ops._transformed())):
+                or self.sparse or type(w) not in (torch.Tensor, nn.Parameter) or type(ids) is not torch.Tensor
+                or (not torch.compiler.is_compiling() and ops._transformed())):
             out = super().forward(ids)
             return out if self.scale == 1.0 else out * self.scale
         return ops.embedding(ids, w, self.scale, self.padding_idx)

@@ -259,3 +259,31 @@ def test_module_under_transforms():
     out = e(ids)
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         torch.autograd.grad(out, e.weight, forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def test_module_with_a_table_of_another_kind():
+    """A tensor subclass that answers torch's own operators alone, as sharded tables do, keeps them."""
+    import hawk_b200.model as M
+
+    class Table(torch.Tensor):
+        @staticmethod
+        def __new__(cls, data):
+            return torch.Tensor._make_wrapper_subclass(cls, data.shape, dtype=data.dtype, device=data.device)
+
+        def __init__(self, data):
+            self.data_of = data
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            if func.namespace != "aten":
+                raise NotImplementedError(str(func))
+            plain = lambda a: a.data_of if isinstance(a, Table) else a  # noqa: E731
+            out = func(*(plain(a) for a in args), **{k: plain(a) for k, a in (kwargs or {}).items()})
+            return Table(out) if func is torch.ops.aten.detach.default else out
+
+    data, ids = torch.randn(7, 4, device="cuda"), torch.tensor([6, 0, 6], device="cuda")
+    e = M.Embedding(7, 4, scale=3.0)
+    e.weight = torch.nn.Parameter(Table(data), requires_grad=False)
+    assert torch.equal(e(ids), data[ids] * 3.0)
+    e.weight = torch.nn.Parameter(data, requires_grad=False)
+    assert torch.equal(e(ids.as_subclass(type("Ids", (torch.Tensor,), {}))), data[ids] * 3.0)

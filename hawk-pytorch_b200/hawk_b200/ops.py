@@ -2013,14 +2013,14 @@ embedding_fwd.register_autograd(_embed_backward, setup_context=_embed_setup)
 
 
 def _embed_bwd_setup(ctx, inputs, output):
-    ids, _, V, ctx.scale, ctx.padding_idx = inputs
+    ids, _, ctx.V, ctx.scale, ctx.padding_idx = inputs
     ctx.save_for_backward(ids)
 
 
-def _embed_bwd_backward(ctx, ddw):  # linear in dout: its rows are those of ddw, nothing where padding_idx kept one out
+def _embed_bwd_backward(ctx, ddw):  # linear in dout: its rows are those of ddw, nothing at padding_idx and ids outside the table
     ids, = ctx.saved_tensors
     rows = embedding_fwd(ids, ddw, ctx.scale)
-    return None, rows.masked_fill((ids == ctx.padding_idx)[..., None], 0.0), None, None, None
+    return None, rows.masked_fill(((ids == ctx.padding_idx) | (ids < 0) | (ids >= ctx.V))[..., None], 0.0), None, None, None
 
 
 embedding_bwd.register_autograd(_embed_bwd_backward, setup_context=_embed_bwd_setup)

@@ -287,3 +287,18 @@ def test_module_with_a_table_of_another_kind():
     assert torch.equal(e(ids), data[ids] * 3.0)
     e.weight = torch.nn.Parameter(data, requires_grad=False)
     assert torch.equal(e(ids.as_subclass(type("Ids", (torch.Tensor,), {}))), data[ids] * 3.0)
+
+
+def test_gradient_of_the_gradient_outside_the_table():
+    """Positions that have no part in the table's gradient have none in its derivative."""
+    from hawk_b200 import embedding
+    w = torch.randn(6, 4, device="cuda", requires_grad=True)
+    ids = torch.tensor([1, -1, 6, 2 ** 40, 5, 0, -6], device="cuda")
+    out = embedding(ids, w, 2.0, padding_idx=0)
+    go = torch.randn(7, 4, device="cuda").requires_grad_()
+    dw, = torch.autograd.grad(out, w, go, create_graph=True)
+    u = torch.randn_like(dw)
+    dgo, = torch.autograd.grad(dw, go, u)
+    want = torch.zeros(7, 4, device="cuda")
+    want[0], want[4] = 2.0 * u[1], 2.0 * u[5]
+    assert torch.equal(dgo, want)

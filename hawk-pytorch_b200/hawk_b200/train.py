@@ -35,7 +35,8 @@ def init_distributed(backend: Optional[str] = None) -> tuple:
 def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
     """Scales the gradients of `parameters` (fp32 or bf16, on one CUDA device) in place so that their global 2-norm is at most
     `max_norm`, by torch.nn.utils.clip_grad_norm_'s rule: times min(1, max_norm / (norm + 1e-6)).  Returns the norm before, as a
-    scalar on the device; nothing synchronises.  `FusedAdamW(max_grad_norm=)` does the same without a pass of its own."""
+    scalar on the device; nothing synchronises.  Contiguous gradients that share memory are refused before any is scaled.
+    `FusedAdamW(max_grad_norm=)` does the same without a pass of its own."""
     from . import ops
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads, seen = [], set()
@@ -45,13 +46,17 @@ def clip_grad_norm_(parameters, max_norm: float) -> torch.Tensor:
             grads.append(p.grad)
     if not grads:
         return torch.zeros(())
+    if any(n > 1 and s == 0 for g in grads if g.numel() for n, s in zip(g.shape, g.stride())):
+        raise ValueError("hawk_b200: a gradient whose elements share memory (an expanded one) cannot be scaled in place")
     with torch.no_grad():
-        table, device, keep = ops._norm_table(grads)
+        # strided gradients go through a copy, so that whatever memory they share with others is scaled once
+        dense = [g if g.is_contiguous() else g.contiguous() for g in grads]
+        table, device, keep = ops._norm_table(dense)
         both = ops._grad_norm(table, device, float(max_norm))
-        ops.scale_in_place([g for g in grads if g.is_contiguous()], both[1])  # first: it refuses gradients that share memory
-        strided = [g for g in grads if not g.is_contiguous()]
-        if strided:  # torch's own product, which knows strides
-            torch._foreach_mul_(strided, both[1])
+        ops.scale_in_place(dense, both[1])
+        for g, d in zip(grads, dense):
+            if d is not g:
+                g.copy_(d)
     return both[0]
 
 

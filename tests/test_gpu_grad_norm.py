@@ -246,3 +246,51 @@ def test_views_of_a_flat_buffer(n, dtype):
         half = torch.finfo(dtype).eps / 2
         assert bool(((v.double() - want * 0.37).abs() <= (half + 2 * 2.0 ** -24) * want.abs() * 0.37).all())
         assert bool(flat[:off].isnan().all()) and bool(flat[off + n:].isnan().all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strided_gradients_get_the_same_factor(dtype):
+    """A factor that bf16 does not hold (0.37), on gradients of every layout: one rounding each."""
+    from hawk_b200.train import clip_grad_norm_
+    torch.manual_seed(2)
+    flat = torch.randn(40, 96, device="cuda").to(dtype)
+    ps = [torch.nn.Parameter(torch.zeros(s, dtype=dtype, device="cuda")) for s in ((40, 32), (40, 32), (48, 33), (7, 5, 3), (0, 4))]
+    ps[0].grad, ps[1].grad = flat[:, ::3], flat[:, 1::3]  # interleaved, but without an element in common
+    ps[2].grad = torch.randn(33, 48, device="cuda").to(dtype).t()
+    ps[3].grad = torch.randn(3, 5, 7, device="cuda").to(dtype).permute(2, 1, 0)
+    ps[4].grad = torch.zeros(4, 0, dtype=dtype, device="cuda").t()
+    had, between = [p.grad.clone() for p in ps], flat[:, 2::3].clone()
+    norm = _norm64(had)
+    layouts = [(p.grad.data_ptr(), p.grad.stride(), p.grad._version) for p in ps[:4]]
+    assert abs(float(clip_grad_norm_(ps, 0.37 * norm)) - norm) <= 1e-6 * norm
+    for p, h, (at, stride, version) in zip(ps, had, layouts):
+        want = h.double() * (0.37 * norm / (norm + 1e-6))
+        assert bool(((p.grad.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 4 * 2.0 ** -24) * want.abs()).all())
+        assert (p.grad.data_ptr(), p.grad.stride()) == (at, stride) and p.grad._version > version
+    assert torch.equal(flat[:, 2::3], between)
+
+
+def test_strided_gradients_that_share_memory_are_scaled_once():
+    from hawk_b200.train import clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(8, 8, device="cuda")) for _ in range(3)]
+    shared = torch.ones(8, 8, device="cuda").t()
+    flat = torch.ones(8, 8, device="cuda")
+    shared[0, 1] = 2.0  # not its own transpose
+    ps[0].grad = ps[1].grad = shared
+    ps[2].grad = torch.ones(8, 16, device="cuda")[:, ::2]
+    more = [torch.nn.Parameter(torch.zeros(s, device="cuda")) for s in ((8, 8), (4, 8))]
+    more[0].grad, more[1].grad = flat, flat[::2]  # a contiguous one and a strided view of it
+    had = [p.grad.clone() for p in ps + more]
+    norm = _norm64(had)
+    clip_grad_norm_(ps + more, norm / 4)
+    for p, h in zip(ps + more, had):
+        assert torch.allclose(p.grad, h * 0.25, rtol=1e-6)
+
+
+def test_a_clip_that_cannot_be_written_changes_nothing():
+    from hawk_b200.train import clip_grad_norm_
+    ps = [torch.nn.Parameter(torch.zeros(8, 8, device="cuda")) for _ in range(2)]
+    ps[0].grad, ps[1].grad = torch.ones(8, 8, device="cuda"), torch.ones(8, 1, device="cuda").expand(8, 8)
+    with pytest.raises(ValueError, match="share memory"):
+        clip_grad_norm_(ps, 0.5)
+    assert all(bool((p.grad == 1).all()) for p in ps)

@@ -2109,7 +2109,7 @@ def grad_norm(tensors) -> torch.Tensor:
 
 
 def scale_in_place(tensors, scale: torch.Tensor) -> None:
-    """t *= scale for every t of `tensors` (fp32 or bf16, contiguous, not overlapping), with `scale` an fp32 scalar on their
+    """t *= scale for every t of `tensors` (fp32 or bf16, contiguous, not overlapping), with `scale` an fp32 scalar of its own on their
     device; nothing is read or written where it is 1."""
     tensors = list(tensors)
     if not all(map(_tensor.is_contiguous, tensors)):
@@ -2122,6 +2122,8 @@ def scale_in_place(tensors, scale: torch.Tensor) -> None:
         raise ValueError("hawk_b200: tensors that share memory cannot be scaled in place by one call")
     if scale.device != device or scale.dtype != torch.float32 or scale.numel() != 1:
         raise ValueError(f"hawk_b200: scale has to be an fp32 scalar on {device}")
+    if any(a < scale.data_ptr() + 4 and scale.data_ptr() < b for a, b in spans):
+        raise ValueError("hawk_b200: the scale cannot share memory with a tensor that it scales")
     lib = _lib.load()
     count = len(table) // 3
     with _on(scale, "scale_multi", (count + 1023) // 1024):

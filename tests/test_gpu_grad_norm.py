@@ -294,3 +294,13 @@ def test_a_clip_that_cannot_be_written_changes_nothing():
     with pytest.raises(ValueError, match="share memory"):
         clip_grad_norm_(ps, 0.5)
     assert all(bool((p.grad == 1).all()) for p in ps)
+
+
+def test_a_factor_among_the_scaled_is_refused():
+    from hawk_b200 import ops
+    x = torch.full((9,), 2.0, device="cuda")
+    for ts, scale in (([x], x[3]), ([x], x[:1]), ([torch.ones(4, device="cuda"), x], x[8])):
+        with pytest.raises(ValueError, match="share memory"):
+            ops.scale_in_place(ts, scale)
+    ops.scale_in_place([x[:8]], x[8])  # beside it is well
+    assert x.tolist() == [4.0] * 8 + [2.0]

@@ -127,13 +127,13 @@ extern "C" int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int cou
   return HAWK_OK;
 }
 
-extern "C" int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
+extern "C" int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, double beta1, double beta2, float eps,
                                 float weight_decay, int64_t step, void* stream) {
   return hawk_adamw_multi_scaled(tensors, count, lr, beta1, beta2, eps, weight_decay, step, nullptr, stream);
 }
 
 extern "C" int hawk_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, float lr,
-                               float beta1, float beta2, float eps, float weight_decay, int64_t step, void* stream) {
+                               double beta1, double beta2, float eps, float weight_decay, int64_t step, void* stream) {
   const hawk_adamw_tensor one = {p, g, m, v, p_bf16, n};
   return hawk_adamw_multi(&one, 1, lr, beta1, beta2, eps, weight_decay, step, stream);
 }

@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_HERE, "libhawk_b200.so")
 
 HAWK_F32 = 0
 HAWK_BF16 = 1
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 _P = c_void_p
 
@@ -57,8 +57,8 @@ SIGNATURES = {
     "hawk_decode_layer_workspace_bytes": (c_size_t, [c_int] * 5),
     "hawk_decode_layer": (c_int, [ctypes.POINTER(DecodeLayerArgs), _P]),
     "hawk_decode_norm_linear": (c_int, [_P, _P, _P, c_float, _P, _P, _P, c_size_t] + [c_int] * 6 + [_P, _P]),
-    "hawk_adamw_step": (c_int, [_P, _P, _P, _P, _P, c_int64, c_float, c_float, c_float, c_float, c_float, c_int64, _P]),
-    "hawk_adamw_multi": (c_int, [c_char_p, c_int, c_float, c_float, c_float, c_float, c_float, c_int64, _P]),
+    "hawk_adamw_step": (c_int, [_P, _P, _P, _P, _P, c_int64, c_float, c_double, c_double, c_float, c_float, c_int64, _P]),
+    "hawk_adamw_multi": (c_int, [c_char_p, c_int, c_float, c_double, c_double, c_float, c_float, c_int64, _P]),
     "hawk_adamw_multi_scaled": (c_int, [c_char_p, c_int, c_float, c_double, c_double, c_float, c_float, c_int64, _P, _P]),
     "hawk_grad_norm_workspace_bytes": (c_size_t, [c_int]),
     "hawk_grad_norm": (c_int, [c_char_p, c_int, c_float, _P, _P, c_size_t, _P]),

@@ -28,7 +28,7 @@
 extern "C" {
 #endif
 
-#define HAWK_B200_ABI_VERSION 7
+#define HAWK_B200_ABI_VERSION 8
 
 typedef enum hawk_dtype { HAWK_F32 = 0, HAWK_BF16 = 1 } hawk_dtype;
 
@@ -360,9 +360,10 @@ int hawk_scale(const float* src, const float* scale, void* dst, int64_t n, int d
  * step number `step` >= 1) on n contiguous fp32 elements, in place in p, m (first moment) and v (second
  * moment); g is the gradient.  p_bf16 (may be NULL) receives the bf16 rounding of the updated p, so the
  * next forward needs no cast pass.  No counterpart in the reference, which stops at loss.backward()
- * (README.md:36) and leaves the optimiser to the user; this is the update torch.optim.AdamW would make. */
-int hawk_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, float lr, float beta1,
-                    float beta2, float eps, float weight_decay, int64_t step, void* stream);
+ * (README.md:36) and leaves the optimiser to the user; this is the update torch.optim.AdamW would make.
+ * The betas are doubles: 1 - beta, formed from a beta rounded to fp32, would be 1.3e-5 off at 0.999. */
+int hawk_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, int64_t n, float lr, double beta1,
+                    double beta2, float eps, float weight_decay, int64_t step, void* stream);
 /* The same for `count` tensors (a host array) in one launch per 64 of them. */
 typedef struct hawk_adamw_tensor {
   float* p;
@@ -371,10 +372,9 @@ typedef struct hawk_adamw_tensor {
   void* p_bf16; /* NULL: no bf16 copy */
   int64_t n;
 } hawk_adamw_tensor;
-int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, float beta1, float beta2, float eps,
+int hawk_adamw_multi(const hawk_adamw_tensor* tensors, int count, float lr, double beta1, double beta2, float eps,
                      float weight_decay, int64_t step, void* stream);
-/* The same with the gradients taken times *grad_scale (a device scalar, e.g. the second result of hawk_grad_norm; NULL = 1).
- * The betas are doubles: 1 - beta, formed from a beta rounded to fp32, would be 1.3e-5 off at 0.999. */
+/* The same with the gradients taken times *grad_scale (a device scalar, e.g. the second result of hawk_grad_norm; NULL = 1). */
 int hawk_adamw_multi_scaled(const hawk_adamw_tensor* tensors, int count, float lr, double beta1, double beta2, float eps,
                             float weight_decay, int64_t step, const float* grad_scale, void* stream);
 

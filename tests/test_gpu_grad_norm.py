@@ -304,3 +304,31 @@ def test_a_factor_among_the_scaled_is_refused():
             ops.scale_in_place(ts, scale)
     ops.scale_in_place([x[:8]], x[8])  # beside it is well
     assert x.tolist() == [4.0] * 8 + [2.0]
+
+
+def test_every_adamw_entry_point_forms_the_same_update():
+    import struct
+
+    from hawk_b200 import _lib
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    torch.manual_seed(4)
+    first = [torch.randn(1000, device="cuda") for _ in range(2)] + [torch.zeros(1000, device="cuda") for _ in range(2)]
+    rest = (1e-3, 0.9, 0.999, 1e-8, 0.1)
+    got = []
+    for entry in ("scaled", "multi", "step"):
+        p, g, m, v = (t.clone() for t in first)
+        for step in (1, 2, 3):
+            one = struct.pack("6Q", *(t.data_ptr() for t in (p, g, m, v)), 0, 1000)
+            if entry == "scaled":
+                rc = lib.hawk_adamw_multi_scaled(one, 1, *rest, step, None, st)
+            elif entry == "multi":
+                rc = lib.hawk_adamw_multi(one, 1, *rest, step, st)
+            else:
+                rc = lib.hawk_adamw_step(p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), None, 1000, *rest, step, st)
+            assert rc == 0
+        got.append((p, m, v))
+    g = first[1].double()
+    # v after three equal gradients: g^2 (1 - beta^3), three roundings a step
+    assert float((got[0][2].double() / (g * g * (1 - 0.999 ** 3)) - 1).abs().max()) <= 12 * 2.0 ** -24
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))

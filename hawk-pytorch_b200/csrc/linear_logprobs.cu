@@ -18,10 +18,13 @@
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
 //      probability, g_lp (1 - p) as -expm1 (log p_j of the others is that of the rounded e_j, 2^-12 off: where the two terms of a
 //      small vocabulary nearly cancel, that much of g_H p_j is left); bf16 for the products, out of place: a second backward finds e as it was.  The token's
-//      element is most of its row, so the row is first scaled, by 2^-8 at most, to where that element is a bf16 number, and d act's
+//      element is most of its row, so the row is first scaled, by up to 2, to where that element is a bf16 number, and d act's
 //      row is scaled back as it leaves the product: its error is then that of its own rounding alone (1.7e-3 in norm where two
-//      roundings left 2.4e-3).  d W takes the rows as they are, which is the element's own rounding; few rows it
-//      takes twice, as two bf16 numbers to each of fp32 (kTwiceRows).
+//      roundings left 2.4e-3).  d W takes the row's activations scaled back, a copy rounded to bf16 once more.  Each row has a scale
+//      of its own (dithered): where the upstream gradients are alike (a mean), so are the tokens' elements, and one scale
+//      for all, the nearest bf16 number's, would leave a common factor in the whole d W (0.34 % at 255 rows if the activations stayed as
+//      they are, 0.09 % with them scaled back, since they lie on bf16's grid), where independent roundings average out.  Few
+//      rows d W takes twice, as two bf16 numbers to each of fp32, from a scale within 2^-8 of 1 (kTwiceRows).
 //   4. two GEMMs, d act = dx W and d W = dx^T act; d act's rows go back to their places.
 // Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16, all rows named:
 // 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.3 ms (1.36; dx 0.7 at 5.9 TB/s, the
@@ -38,14 +41,14 @@ struct ScoreRows {
   int64_t* token;    // [N] compact row -> token (>= 0)
 };
 // The d W product reads whole K blocks of BK compact rows, zeros behind the last one.  Where few rows are named it reads each twice: as
-// many rows follow with what rounding d x to bf16 left, and act again.  (Sums of few terms do not average their roundings: d W
+// many rows follow with what rounding d x to bf16 left, and act again, as it is.  (Sums of few terms do not average their roundings: d W
 // of 8 to 64 rows was 1.2 to 1.76 times as far off as a single rounding leaves it, and is 1.00 now; from 200 rows on 1.35 to 1.5, in
 // thousands 1.41 to 1.46.  The backward of 31 / 128 rows at H2048 V32000 takes 93 / 106 us instead of 88 / 96.)
 constexpr int kTwiceRows = 128;
 __host__ __device__ constexpr int64_t whole_blocks(int64_t rows) { return (rows + BK - 1) / BK * BK; }
 __device__ __forceinline__ int padded_count(int count) { return (int)whole_blocks(max(count, 1)); }
 __device__ __forceinline__ bool twice(int count) { return count <= kTwiceRows; }
-// rows that d x and the compact act have room for
+// rows that d x and the activations beside it have room for
 __host__ __device__ constexpr int64_t room_rows(int64_t N) {
   return whole_blocks(N) > 2 * kTwiceRows ? whole_blocks(N) : 2 * whole_blocks(N) < 2 * kTwiceRows ? 2 * whole_blocks(N) : 2 * kTwiceRows;
 }
@@ -133,23 +136,14 @@ score_prepare_kernel(const int64_t* __restrict__ tokens, const T* __restrict__ a
   }
 }
 
-// a warp to a compact row; `act` compact, and completed as far as the d W product reads
+// a warp to a compact row; `act` compact
 __global__ void __launch_bounds__(256)
 score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ correct, ScoreRows rows,
-                    const __nv_bfloat16* __restrict__ weight, __nv_bfloat16* __restrict__ act, float* __restrict__ logprob,
+                    const __nv_bfloat16* __restrict__ weight, const __nv_bfloat16* __restrict__ act, float* __restrict__ logprob,
                     float* __restrict__ entropy, float2* __restrict__ stats, int H, int V, int groups,
                     const int* __restrict__ status) {
-  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, count = *rows.count;
-  if (r < padded_count(count)) {
-    uint4* again = twice(count) ? reinterpret_cast<uint4*>(act + (long long)(padded_count(count) + r) * H) : nullptr;
-    uint4* here = reinterpret_cast<uint4*>(act + (long long)r * H);
-    for (int i = lane; i < H / 8; i += 32) {
-      const uint4 v = r < count ? here[i] : make_uint4(0u, 0u, 0u, 0u);
-      if (r >= count) here[i] = v;
-      if (again) again[i] = v;
-    }
-  }
-  if (r >= count) return;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= *rows.count) return;
   const float4* g = score + (long long)r * groups;
   const int64_t token = rows.token[r];
   float own = 0.f;
@@ -200,15 +194,61 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
   }
 }
 
+// the bf16 number of v's sign and exponent whose mantissa is row r's: 7 bits of a multiple of the golden ratio, evenly spread
+__device__ __forceinline__ float dithered(float v, uint32_t r) {
+  return __uint_as_float((__float_as_uint(v) & 0xff800000u) | r * 2654435769u >> 25 << 16);
+}
+
+// the token's element of d x and what it is stored as: where it is exact in bf16 the row is scaled by own16 / own
+struct TokenElement {
+  float own, own16, shrink, grow;
+  __device__ __forceinline__ TokenElement(float lp, float H, float gl, float gh, uint32_t r, bool two) {
+    own = fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H));
+    const bool scaled = fabsf(own) > 1e-30f && fabsf(own) < 1e37f;
+    own16 = scaled && !two ? dithered(own, r) : __bfloat162float(__float2bfloat16(own));
+    shrink = scaled ? own16 / own : 1.f;
+    grow = scaled ? own / own16 : 1.f;
+  }
+};
+
 // d x of a share of one compact row per block, 8 columns (16 bytes of e, of one group) per vector, all of a thread's requested before
 // what the row's factors are known, pairs of fp32 operations, and no call in the loop.  16380 rows of 32000: 355 us (5.9 TB/s), 1548 rows 36;
-// a row to a block of 512 threads in a loop with the token's element among the others 403 and 42
+// a row to a block of 512 threads in a loop with the token's element among the others 403 and 42.
+// The blocks behind write the activations that the d W product takes with it, a warp to a row (3108 rows of 2048: 3 us more, by the
+// first block of each row 10).
 constexpr int kDxThreads = 256, kDxVectors = 4, kDxShare = kDxThreads * kDxVectors;
 __global__ void __launch_bounds__(kDxThreads)
 score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, const float2* __restrict__ stats,
                 const float* __restrict__ logprob, const float* __restrict__ entropy, ScoreRows rows,
                 const float* __restrict__ g_lp, const float* __restrict__ g_ent, __nv_bfloat16* __restrict__ dx, float* __restrict__ row_scale,
-                long long ld, int V, int groups, uint32_t shares) {
+                const __nv_bfloat16* __restrict__ act, __nv_bfloat16* __restrict__ dw_act, long long ld, int V, int width, int groups,
+                uint32_t shares, uint32_t dx_blocks) {
+  if (blockIdx.x >= dx_blocks) {
+    const int r = (int)(blockIdx.x - dx_blocks) * 8 + (int)(threadIdx.x >> 5), count = *rows.count, padded = padded_count(count);
+    if (r >= padded) return;
+    const bool named = r < count, two = twice(count);
+    const int row = named ? rows.row[r] : 0;
+    const TokenElement t(logprob[row], entropy[row], g_lp ? g_lp[row] : 0.f, g_ent ? g_ent[row] : 0.f, r, two);
+    const uint4* from = reinterpret_cast<const uint4*>(act + (long long)r * width);
+    uint4* to = reinterpret_cast<uint4*>(dw_act + (long long)r * width);
+    uint4* again = reinterpret_cast<uint4*>(dw_act + (long long)(padded + r) * width);
+#pragma unroll 4
+    for (int i = threadIdx.x & 31; i < width / 8; i += 32) {
+      uint4 a = named ? __ldg(from + i) : make_uint4(0u, 0u, 0u, 0u);
+      if (two) {
+        again[i] = a;
+      } else {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&a);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 v = mul2(unpack_bf16x2(w[k]), f2(t.grow));
+          w[k] = pack_bf16x2(v.x, v.y);
+        }
+      }
+      to[i] = a;
+    }
+    return;
+  }
   const uint32_t r = blockIdx.x / shares;
   const int i0 = (int)(blockIdx.x - r * shares) * kDxShare + (int)threadIdx.x;
   const int nvec = (V + 7) / 8;  // ld is a multiple of 8; what lies behind V is never read
@@ -242,9 +282,8 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   const float2 st = stats[r];
   const float lp = logprob[row], H = entropy[row], gl = g_lp ? g_lp[row] : 0.f, gh = g_ent ? g_ent[row] : 0.f;
   const bool known = token < V;
-  const float own = fmaf(-gl, expm1f(lp), -gh * expf(lp) * (lp + H)), own16 = __bfloat162float(__float2bfloat16(own));
-  const bool scaled = fabsf(own) > 1e-30f && fabsf(own16) < 1e37f;
-  const float shrink = scaled ? own16 / own : 1.f, grow = scaled ? own / own16 : 1.f;
+  const TokenElement el(lp, H, gl, gh, r, rest != nullptr);
+  const float own = el.own, own16 = el.own16, shrink = el.shrink, grow = el.grow;
   if (blockIdx.x == r * shares && threadIdx.x == 0) row_scale[r] = grow;
 #pragma unroll
   for (int q = 0; q < kDxVectors; ++q) {
@@ -276,7 +315,7 @@ score_dx_kernel(const __half* __restrict__ e, const float4* __restrict__ score, 
   // the token's own element anew, by the thread that wrote it
   const int64_t in_share = token / 8 - (i0 - (int)threadIdx.x);
   if (known && in_share >= 0 && in_share < kDxShare && (int)threadIdx.x == (int)in_share % kDxThreads) {
-    out[token] = __float2bfloat16(own);
+    out[token] = __float2bfloat16(own16);
     if (rest) rest[token] = __float2bfloat16(own - own16);
   }
 }
@@ -356,7 +395,7 @@ static ScoreSaved score_saved(long long N, long long H, long long V, int w_dtype
   L.groups = (int)((V + EPI_COLS - 1) / EPI_COLS);
   size_t o = 0;
   L.wb = o;      o += w_dtype == HAWK_F32 ? up256((size_t)V * H * 2) : 0;
-  L.ab = o;      o += up256((size_t)room_rows(N) * H * 2);
+  L.ab = o;      o += up256((size_t)N * H * 2);
   L.count = o;   o += 256;
   L.row = o;     o += up256((size_t)N * 4);
   L.token = o;   o += up256((size_t)N * 8);
@@ -372,7 +411,7 @@ static ScoreRows score_rows(const ScoreSaved& S, const void* saved) {
   return ScoreRows{reinterpret_cast<int*>(p + S.count), reinterpret_cast<int*>(p + S.row), reinterpret_cast<int64_t*>(p + S.token)};
 }
 struct ScoreScratch {
-  size_t dx, row_scale, partial, total;
+  size_t dx, row_scale, act, partial, total;
 };
 // d act of up to this many rows leaves partial sums in fp32 over splits of K that its kernel plans for the rows that are named (3108 rows
 // of 2048, V32000, nine of ten left out: backward 386 -> 143 us, half 519 -> 393); of more rows even a tenth fills the GPU, and their product leaves what it is
@@ -387,6 +426,7 @@ static ScoreScratch score_scratch(long long N, long long H, long long V, bool wa
   size_t o = 0, part = 0;
   L.dx = o;      o += up256((size_t)room_rows(N) * ((V + 7) & ~7LL) * 2);
   L.row_scale = o; o += up256((size_t)N * 4);
+  L.act = o;     o += want_dw ? up256((size_t)room_rows(N) * H * 2) : 0;
   if (want_da) part = (size_t)std::max<int64_t>(N, da_part_rows(N, plan_grad(N, H, V))) * H * 4;  // its compact rows, in fp32 at most
   const long long splits = want_dw ? plan_grad(V, H, room_rows(N)).splits : 1;
   if (splits > 1) part = std::max<size_t>(part, (size_t)splits * V * H * 4);
@@ -476,7 +516,7 @@ extern "C" int hawk_linear_logprobs(const void* weight, const void* act, const i
   else
     rc = launch_gemm<EPI_SCORE, 1, false, false>(ab, H, wb, H, nullptr, false, S.ldV, (int)N, (int)V, (int)H, 1, ep, status, st);
   if (rc != HAWK_OK) return rc;
-  score_reduce_kernel<<<(unsigned)(whole_blocks(N) / 8), 256, 0, st>>>(ep.score, correct, rows, wb, ab, logprob, entropy,
+  score_reduce_kernel<<<(unsigned)((N + 7) / 8), 256, 0, st>>>(ep.score, correct, rows, wb, ab, logprob, entropy,
                                                                reinterpret_cast<float2*>(sv + S.stats), (int)H, (int)V, S.groups,
                                                                status);
   return launch_status();
@@ -493,7 +533,7 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const ScoreSaved S = score_saved(N, H, V, w_dtype, true);
   const ScoreScratch L = score_scratch(N, H, V, dweight != nullptr, dact != nullptr);
   HAWK_REQUIRE(saved && saved_bytes >= S.total && scratch && scratch_bytes >= L.total, HAWK_ERR_WORKSPACE);
-  HAWK_REQUIRE(N * (H / 256 + 1) < (1LL << 31) && whole_blocks(N) * (V / (8 * kDxShare) + 1) < (1LL << 31), HAWK_ERR_SHAPE);
+  HAWK_REQUIRE(N * (H / 256 + 1) < (1LL << 31) && whole_blocks(N) * (V / (8 * kDxShare) + 2) < (1LL << 31), HAWK_ERR_SHAPE);
   HAWK_REQUIRE(aligned(saved, 256) && aligned(scratch, 256) && aligned(dweight, 16) && aligned(dact, 16) && aligned(weight, 16) &&
                    aligned(act, 16) && aligned(tokens, 8) && aligned(logprob, 4) && aligned(entropy, 4) && aligned(g_logprob, 4) &&
                    aligned(g_entropy, 4),
@@ -506,17 +546,19 @@ extern "C" int hawk_linear_logprobs_bwd(const void* weight, const void* act, con
   const ScoreRows rows = score_rows(S, saved);
   auto* dx = reinterpret_cast<__nv_bfloat16*>(sc + L.dx);
   auto* row_scale = reinterpret_cast<float*>(sc + L.row_scale);
+  auto* dw_act = reinterpret_cast<__nv_bfloat16*>(sc + L.act);
   auto* part = reinterpret_cast<float*>(sc + L.partial);
   const int64_t shares = ((V + 7) / 8 + kDxShare - 1) / kDxShare;
-  score_dx_kernel<<<(unsigned)(whole_blocks(N) * shares), kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
+  const int64_t dx_blocks = whole_blocks(N) * shares, act_blocks = dweight ? whole_blocks(N) / 8 : 0;
+  score_dx_kernel<<<(unsigned)(dx_blocks + act_blocks), kDxThreads, 0, st>>>(reinterpret_cast<const __half*>(sv + S.e),
                                                                  reinterpret_cast<const float4*>(sv + S.score),
                                                                  reinterpret_cast<const float2*>(sv + S.stats), logprob, entropy, rows,
-                                                                 g_logprob, g_entropy, dx, row_scale, S.ldV, (int)V, S.groups,
-                                                                 (uint32_t)shares);
+                                                                 g_logprob, g_entropy, dx, row_scale, ab, dw_act, S.ldV, (int)V, (int)H,
+                                                                 S.groups, (uint32_t)shares, (uint32_t)dx_blocks);
   rc = launch_status();
   if (rc != HAWK_OK) return rc;
-  if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the compact rows of dx and act are the K index)
-    rc = grad_gemm<true, true>(dx, S.ldV, ab, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)room_rows(N), rows.count + 1, part, status, st);
+  if (dweight) {  // d weight [V,H] = dx^T . act [N,H]: A and B MN-major (the compact rows of dx and their activations are the K index)
+    rc = grad_gemm<true, true>(dx, S.ldV, dw_act, H, dweight, dw_dtype, nullptr, (int)V, (int)H, (int)room_rows(N), rows.count + 1, part, status, st);
     if (rc != HAWK_OK) return rc;
   }
   if (dact) {  // d act [N,H] = dx [N,V] . W [V,H]: A K-major, B MN-major (W's rows are the K index); compact rows

@@ -1883,8 +1883,7 @@ def _(weight, act, tokens, want_grad):
     (V, H), N = weight.shape, tokens.numel()
     up = lambda n: (n + 255) // 256 * 256  # noqa: E731
     n = up(N * ((V + 127) // 128) * 16) + 2 * up(N * 8) + 2 * up(N * 4) + 256 + (up(N * ((V + 7) // 8 * 8) * 2) if want_grad else 0)
-    whole = (N + 63) // 64 * 64
-    n += up(max(whole, min(2 * whole, 256)) * H * 2) + (up(V * H * 2) if weight.dtype == torch.float32 else 0)
+    n += up(N * H * 2) + (up(V * H * 2) if weight.dtype == torch.float32 else 0)
     return (*(act.new_empty(tokens.shape, dtype=torch.float32) for _ in range(2)), act.new_empty(n, dtype=torch.uint8))
 
 

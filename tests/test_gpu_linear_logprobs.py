@@ -329,3 +329,24 @@ def test_activations_gradient_of_many_rows(N, dtype):
     w, a, t, gl, ge = _case(N, 64, 1000, 18, dtype)
     for every in (1, 2, 40):
         _check(w, a, torch.where(torch.arange(N, device="cuda") % every == 0, t, -1), gl, ge)
+
+
+@pytest.mark.parametrize("w_dtype", [F32, BF16])
+@pytest.mark.parametrize("N", [100, 129, 255, 1548])
+def test_gradients_of_a_mean(N, w_dtype):
+    """Upstream gradients alike in every row: no rounding may turn into a common factor.  With N >= 100 rows, H = 64 and 2000 tokens the
+    weight's gradient takes at least N H = 6400 independent roundings of at most 2^-8, so its component along the true one is off by
+    2^-8 / sqrt(3 N H) = 3e-5 in the mean square; 2^-11 is 17 times that.  As a whole it is off by two roundings of operands and, in bf16,
+    its own: sqrt(3) 2^-8 / sqrt(3) in norm at most."""
+    from hawk_b200 import linear_logprobs
+    w, a, t, _, _ = _case(N, 64, 2000, N, w_dtype=w_dtype, lift=0.0)
+    w, a = w.detach().requires_grad_(), a.detach().requires_grad_()
+    lp, H = linear_logprobs(w, a, t)
+    gl = torch.full((N,), -1.0 / N, device="cuda")
+    dw, da = torch.autograd.grad(lp, (w, a), gl)
+    _, _, rdw, rda = _reference(w.detach(), a.detach(), t, gl, torch.zeros_like(gl))
+    named = torch.zeros(2000, dtype=torch.bool, device="cuda").index_fill_(0, t, True)
+    for got, want in ((dw[named], rdw[named]), (dw[~named], rdw[~named]), (da, rda)):
+        factor = float((got.double() * want).sum() / (want * want).sum())
+        assert abs(factor - 1) <= 2.0 ** -11, factor
+        assert rel_l2(got, want) <= 2.0 ** -8

@@ -20,6 +20,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "tc05.cuh"
 
@@ -56,7 +57,7 @@ struct EpiParams {
   float* correct;            // [M] logit at the label
   const long long* labels;   // [M]
   // EPI_SCORE, EPI_SCORE_KEEP (which also stores e^(x - max) in fp16): `correct` and `labels` as above, and
-  float4* score;             // [M, column groups of 128] (max, sum exp, sum exp (x - max) log2 e, unused)
+  float4* score;             // [M, column groups of 128] (max, sum exp without `ties`, sum exp (x - max) log2 e, ties)
   int groups;                // column groups
   // EPI_OUT
   int out_bf16;              // the store map's type
@@ -121,10 +122,11 @@ __device__ __forceinline__ void softmax_chunk(const uint32_t (&v)[32], int cbase
 }
 
 // One 32-column chunk of unrounded logits of one row, whose group's maximum m is known: the sums of e = e^(x - m) and of
-// e (x - m) log2 e (for the entropy), the label's logit, and with KEEP e itself in fp16 (at most 1, so nothing overflows).
-template <bool FULL, bool KEEP>
-__device__ __forceinline__ void score_chunk(const uint32_t (&v)[32], float m, int cbase, int Nc, long long label, float* correct,
-                                            uint32_t (&packed)[16], float2& s, float2& sx) {
+// e (x - m) log2 e (for the entropy), the label's logit, and with KEEP e itself in fp16 (at most 1, so nothing overflows).  With APART
+// `rest` is the sum of e without the elements at `apart` (m, or NaN: all of them).
+template <bool FULL, bool KEEP, bool APART>
+__device__ __forceinline__ void score_chunk(const uint32_t (&v)[32], float m, float apart, int cbase, int Nc, long long label, float* correct,
+                                            uint32_t (&packed)[16], float2& s, float2& sx, float2& rest) {
 #pragma unroll
   for (int j = 0; j < 16; ++j) {
     float2 x = make_float2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
@@ -135,6 +137,7 @@ __device__ __forceinline__ void score_chunk(const uint32_t (&v)[32], float m, in
     const float2 t = mul2(add2(x, f2(-m)), f2(kLog2e));
     const float2 e = make_float2(ex2_approx(t.x), ex2_approx(t.y));
     s = add2(s, e);
+    if (APART) rest = add2(rest, make_float2(x.x == apart ? 0.f : e.x, x.y == apart ? 0.f : e.y));
     sx = fma2(e, t, sx);
     if (KEEP) packed[j] = pack_f16x2(e.x, e.y);
   }
@@ -383,7 +386,14 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         }
         const float m = fmaxf(m0, m1);
         const long long label = score_label;
-        float2 s = f2(0.f), sx = f2(0.f);
+        // In a row whose token is all but certain the other elements are what 1 - p is made of, and lost beside its 1.  Where the
+        // odd and the even columns' maxima lie so far apart that the others may be little, the elements at the maximum are kept apart
+        // from the sum, and counted; where they do not, the others are 2^-9 at least, and right to 2^-14 within the sum.
+        const bool lone = fabsf(m0 - m1) > 6.25f;
+        float2 s = f2(0.f), sx = f2(0.f), rest = f2(0.f);
+        const auto sums = [&](auto with) {
+        constexpr bool APART = decltype(with)::value;
+        const float apart = lone ? m : __int_as_float(0x7fc00000);
 #pragma unroll
         for (int c = 0; c < EPI_COLS / 32; ++c) {
           tmem_ld_wait();
@@ -400,9 +410,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
           uint32_t packed[16];
           float* correct = ep.correct + (row_ok ? row : 0);
           if (cbase + 32 <= ep.Nc) {
-            score_chunk<true, KEEP>(v[c & 1], m, cbase, ep.Nc, label, correct, packed, s, sx);
+            score_chunk<true, KEEP, APART>(v[c & 1], m, apart, cbase, ep.Nc, label, correct, packed, s, sx, rest);
           } else if (cbase < ep.Nc) {
-            score_chunk<false, KEEP>(v[c & 1], m, cbase, ep.Nc, label, correct, packed, s, sx);
+            score_chunk<false, KEEP, APART>(v[c & 1], m, apart, cbase, ep.Nc, label, correct, packed, s, sx, rest);
           } else if (KEEP) {  // whole chunk past the vocabulary (same for every lane); the store clips it
 #pragma unroll
             for (int j = 0; j < 16; ++j) packed[j] = 0u;
@@ -414,8 +424,12 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
             if (c & 1) box_store(&map_c, box, lane, col0 + (c >> 1) * 64, row0, 0, ep);
           }
         }
-        if (row_ok && cols > 0)
-          ep.score[(long long)row * ep.groups + col0 / EPI_COLS] = make_float4(m, s.x + s.y, sx.x + sx.y, 0.f);
+        };
+        const bool any = __any_sync(0xffffffffu, lone);
+        if (any) sums(std::true_type{}); else sums(std::false_type{});
+        const float all = s.x + s.y, others = any && lone ? rest.x + rest.y : all;
+        if (row_ok && cols > 0)  // what is apart is a number of ones: the sums' difference but for their rounding
+          ep.score[(long long)row * ep.groups + col0 / EPI_COLS] = make_float4(m, others, sx.x + sx.y, rintf(all - others));
       } else if (MODE == EPI_LOGITS) {
         float run_m = -INFINITY, run_s = 0.f;
         const long long label = row_ok ? ep.labels[row] : -1;

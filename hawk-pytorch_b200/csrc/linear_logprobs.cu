@@ -12,7 +12,8 @@
 //   2. reduce  a warp per row over its groups: m, log s, log probability and entropy.  The token's own logit is formed once more,
 //      as a plain fp32 dot product: the tensor core truncates its running sum at every step of 16 products, which leaves a large
 //      logit a little too small (2e-5 of 16 after 2048 products), and a log probability near 0 would be nothing but that.  The
-//      sums get its term anew as well.  N rows of act and weight read: 50 us of 11 ms at N32760 H2048 V32000.
+//      sums get its term anew as well.  Elements at a group's maximum are counted apart where little else is in their chunk, and
+//      log s is log1p of the rest, so that 1 - p of a token that is all but certain is as exact as the logits.  N rows of act and weight read: 50 us of 11 ms at N32760 H2048 V32000.
 // Backward, from e and the groups' maxima (2 N V bytes kept instead of a third GEMM: forming the logits again takes 2 N H V
 // flops, 3.1 ms at N32760 H2048 V32000 where writing and reading e takes 1):
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
@@ -162,31 +163,48 @@ score_reduce_kernel(const float4* __restrict__ score, const float* __restrict__ 
   for (int i = lane; i < groups; i += 32) m = fmaxf(m, g[i].x);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float s = 0.f, sx = 0.f;
+  float s = 0.f, sx = 0.f, ties = 0.f;  // ties: elements at the row's maximum that their group's sum leaves out
   for (int i = lane; i < groups; i += 32) {
     const float4 v = g[i];
-    const float t = (v.x - m) * kLog2e, k = ex2_approx(t);
-    s = fmaf(v.y, k, s);
+    const float t = (v.x - m) * kLog2e, k = ex2_approx(t), all = v.y + v.w;
+    if (v.x == m) {
+      s += v.y;
+      ties += v.w;
+    } else {
+      s = fmaf(all, k, s);
+    }
     // the group's terms are relative to its own maximum: each moves by t; far below, k is 0 and t finite
-    sx = fmaf(fmaf(v.y, t, v.z), k, sx);
+    sx = fmaf(fmaf(all, t, v.z), k, sx);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, o);
     sx += __shfl_xor_sync(0xffffffffu, sx, o);
+    ties += __shfl_xor_sync(0xffffffffu, ties, o);
     own += __shfl_xor_sync(0xffffffffu, own, o);
   }
   if (lane == 0) {
-    const float nan = __int_as_float(0x7fc00000);
+    const float nan = __int_as_float(0x7fc00000), c = correct[r];
+    float lp = nan, rest = (ties - 1.f) + s, logs = log1pf(rest), base = logs;  // rest: the sum less 1
+    sx *= -0.6931471805599453f;
     if (token < V) {
-      const float t0 = (correct[r] - m) * kLog2e, t1 = (own - m) * kLog2e, e0 = ex2_approx(t0), e1 = ex2_approx(t1);
-      s = (s - e0) + e1;
-      sx = (sx - e0 * t0) + e1 * t1;
-    } else {
-      own = nan;
+      const float d = own - m, t0 = (c - m) * kLog2e, t1 = d * kLog2e, e0 = ex2_approx(t0), e1 = ex2_approx(t1);
+      const bool tied = c == m && ties > 0.f;
+      const float others = tied ? rest : (s - e0) + ties;
+      rest = tied ? rest + expm1f(d) : (ties - 1.f) + ((s - e0) + e1);
+      logs = log1pf(rest);
+      sx += e0 * (c - m);
+      if (d > -1.f) {  // the token has a good part of the sum: from the others, and from where they lie below it
+        lp = -log1pf(others * ex2_approx(-t1));
+        base = -lp;
+        sx = fmaf(others, d, sx);
+      } else {
+        lp = d - logs;
+        base = logs;
+        sx -= e1 * d;
+      }
     }
-    const float logs = logf(s);
-    float lp = (own - m) - logs, ent = logs - 0.6931471805599453f * sx / s;
+    float ent = base + sx / (rest + 1.f);
     if (*status != 0) lp = ent = nan;  // a GEMM gave up a wait (this call's, or an earlier one nobody has looked at)
     logprob[rows.row[r]] = lp;
     entropy[rows.row[r]] = ent;

@@ -350,3 +350,25 @@ def test_gradients_of_a_mean(N, w_dtype):
         factor = float((got.double() * want).sum() / (want * want).sum())
         assert abs(factor - 1) <= 2.0 ** -11, factor
         assert rel_l2(got, want) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("want", [True, False])
+@pytest.mark.parametrize("lift,V", [(30.0, 1000), (30.0, 129), (45.0, 32000)])
+def test_all_but_certain_tokens(lift, V, want):
+    """1 - p and the entropy of tokens whose probability rounds to 1, against their own size.  Each logit is off by 2^-20 of the logits' spread
+    and by half a step of fp32; the terms' sum and log1p add 2^-17: what is left of 1 is off by twice the former and the latter."""
+    from hawk_b200 import linear_logprobs
+    w, a, t, gl, ge = _case(384, 256, V, V, lift=lift)
+    w.requires_grad_(want)
+    lp, H = (x.detach().double() for x in linear_logprobs(w, a, t))
+    logits = a.double() @ w.detach().double().T
+    x = logits.gather(1, t[:, None])
+    others = (logits - x).scatter(1, t[:, None], -math.inf)
+    tail = others.exp().sum(1)                      # (1 - p) / p
+    q = torch.log1p(tail)                           # -log p
+    entropy = q + (torch.where(others.isinf(), 0.0, others) * -(others - q[:, None]).exp()).sum(1)
+    sure = (tail < 0.1) & (tail > 1e-25)
+    assert int(sure.sum()) > 100 and int((tail[sure] < 1e-7).sum()) > 30
+    bound = 2 * (float(logits.abs().max()) * (2.0 ** -20 + 2.0 ** -24)) + 2.0 ** -17
+    assert float((torch.expm1(-lp) / tail - 1).abs()[sure].max()) <= bound
+    assert float((H / entropy - 1).abs()[sure].max()) <= 2 * bound  # its terms hold the logarithm as well

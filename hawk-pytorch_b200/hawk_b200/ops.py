@@ -2101,7 +2101,8 @@ def _grad_norm(table, device, max_norm: float) -> torch.Tensor:
 
 def grad_norm(tensors) -> torch.Tensor:
     """The 2-norm over all elements of `tensors` (fp32 or bf16, any shapes, one device) as an fp32 scalar on their device, in
-    two launches and without a synchronisation.  Not differentiable.  Deterministic, and right for every norm that fp32 can hold
+    two launches and without a synchronisation.  Not differentiable, and a plain function of the tensors' addresses: torch.compile
+    runs it between two graphs, other tracers refuse it.  Deterministic, and right for every norm that fp32 can hold
     (the squares may leave its range)."""
     table, device, keep = _norm_table([tensors] if isinstance(tensors, torch.Tensor) else tensors)
     return _grad_norm(table, device, 0.0)[0]

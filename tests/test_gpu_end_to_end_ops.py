@@ -257,3 +257,32 @@ def test_two_calls_at_once_on_two_streams():
     for k in range(2):
         for out in got[k]:
             assert all(torch.equal(x, y) for x, y in zip(out, want[k]))
+
+
+def test_batched_by_vmap():
+    from hawk_b200 import embedding, linear_logprobs, token_logprobs
+    g = torch.Generator(device="cuda").manual_seed(0)
+    ids = torch.randint(-1, 9, (4, 5), generator=g, device="cuda")
+    w, x, a = (torch.randn(s, generator=g, device="cuda") for s in ((9, 8), (4, 5, 9), (4, 5, 8)))
+    known = ids.clamp(min=0)
+    assert torch.equal(torch.vmap(lambda i: embedding(i, w, 2.0))(known), 2.0 * w[known])
+    assert torch.equal(torch.vmap(lambda v: embedding(known, v))(torch.stack([w, -w])), torch.stack([w[known], -w[known]]))
+    for f, args in ((lambda x, t: token_logprobs(x, t, 2), (x, ids)), (token_logprobs, (x, ids)),
+                    (lambda a, t: linear_logprobs(w, a, t), (a, ids))):
+        assert all(torch.equal(p, q) for p, q in zip(torch.vmap(f)(*args), f(*args)))
+
+
+@pytest.mark.parametrize("op", ["token_logprobs", "linear_logprobs", "embedding"])
+def test_compiled_gradients_are_the_eager_ones(op):
+    import hawk_b200
+    g = torch.Generator(device="cuda").manual_seed(1)
+    ids = torch.randint(0, 300, (4, 50), generator=g, device="cuda")
+    w, x, a = (torch.randn(s, generator=g, device="cuda", requires_grad=True) for s in ((300, 64), (4, 50, 300), (4, 50, 64)))
+    f, leaves = {"token_logprobs": (lambda: sum(hawk_b200.token_logprobs(x, ids - 3)[:2]), (x,)),
+                 "linear_logprobs": (lambda: sum(hawk_b200.linear_logprobs(w, a, ids - 3)), (w, a)),
+                 "embedding": (lambda: hawk_b200.embedding(ids, w, 3.0, 7) * a, (w, a))}[op]
+    results = []
+    for call in (f, torch.compile(f, backend="aot_eager", fullgraph=True)):
+        out = call()
+        results.append([out, *torch.autograd.grad(out, leaves, torch.cos(torch.arange(out.numel(), device="cuda").view(out.shape)))])
+    assert all(torch.equal(p, q) for p, q in zip(*results))

@@ -9,7 +9,8 @@
 //
 // Squares: 16 (fp32) or 32 (bf16) of them are added in fp32, as two sums, and these go to a double.  Where that sum is not well inside
 // fp32's range (over- or underflow of the squares, infinities, NaN) the same elements are squared in double instead, so the
-// norm is right for every list whose norm fp32 can hold.
+// norm is right for every list whose norm fp32 can hold.  Zeros go that way, too, as underflow does (the rows of an embedding's gradient
+// that no token names): 400 M of them in fp32 253 us, as dense ones take, in bf16 146 of 140.
 #include "common.cuh"
 
 namespace hawk {

@@ -57,7 +57,8 @@ __host__ __device__ constexpr int64_t room_rows(int64_t N) {
 // The first row_blocks blocks list `per` rows each (at most one to a thread): a block counts the named tokens before its own by
 // itself, so there is no second launch and no order between blocks.  That is N^2 / (2 per) tokens read from L2 in all: 75 MB at
 // N = 32760, of the 270 that are copied, but 64 ms at 10 M rows; longer lists are counted by block first (`counts`, null otherwise) and
-// a block adds up the counts before its own.  The other blocks cast the weight.
+// a block adds up the counts before its own.  The forward of short rows (H16 V64) without / with the count: 4096 rows 23.6 / 26 us, 16384
+// 35.8 / 35.9, 32768 50 / 46, 65536 81 / 67, 131072 140 / 108.  The other blocks cast the weight.
 constexpr int64_t kCountedRows = 32768;
 __global__ void __launch_bounds__(256) score_count_kernel(const int64_t* __restrict__ tokens, int* __restrict__ counts, int N, int per) {
   const int row = blockIdx.x * per + threadIdx.x;
@@ -432,8 +433,10 @@ struct ScoreScratch {
   size_t dx, row_scale, act, partial, total;
 };
 // d act of up to this many rows leaves partial sums in fp32 over splits of K that its kernel plans for the rows that are named (3108 rows
-// of 2048, V32000, nine of ten left out: backward 386 -> 143 us, half 519 -> 393); of more rows even a tenth fills the GPU, and their product leaves what it is
-// asked for
+// of 2048, V32000, nine of ten left out: backward 386 -> 143 us, half 519 -> 393).  Of more rows the product leaves what it is asked for, as
+// the sums cost where many are named and the splits are fewer in any case: 32760 rows of 2048, d x and d act, planned so / without,
+// all named 3654 / 3558 us, a quarter 1022 / 1002, a tenth 532 / 577, a hundredth 206 / 491.  Just above the border the loss is largest: 8193
+// rows, all 925 / 907, a quarter 388 / 376, a tenth 157 / 347
 constexpr int64_t kPlannedRows = 8192;
 static int da_part_rows(int64_t N, const GradPlan& plan) {  // 0: no partial sums
   const int64_t rows = plan.splits * ((N + 31) / 32 * 32);

@@ -4,7 +4,9 @@
 //   of the last sum are positive),   d x_j = g_lp (onehot_j - p_j) - g_H p_j (log p_j + H).
 // Bound by one read of the logits (the backward: one read, one write).  Measured at 3108 rows of 32000 in bf16: forward 50 us
 // (4.0 TB/s; 72 % of the issue slots and 56 % of the MUFU rate, one exponential per logit), with 20 alternatives 88, backward 64
-// (6.2 TB/s; a torch copy of the same bytes 71); 1551 rows of 31999 in fp32: 46 and 62 us; one row 6 to 8.
+// (6.2 TB/s; a torch copy of the same bytes 71); 1551 rows of 31999 in fp32: 51 and 62 us; one row 6 to 8.
+// Rows left out are not read by the forward (a fifth of the latter: 46 us); the backward requests a row before it knows of its token, and takes
+// as long whatever is left out.
 //
 // Forward: a row belongs to a cluster of 1 to 8 blocks, which split it where there are few rows (one row of 32000 in one block is a
 // chain of 16 16-byte loads per thread).  One pass: every thread keeps its running maximum and the sums relative to it; threads, warps

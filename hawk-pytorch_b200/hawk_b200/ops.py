@@ -1941,8 +1941,8 @@ def linear_logprobs(weight, act, tokens):
     a multiple of 8), both results fp32 of tokens' shape and differentiable in weight and act.  What fused_cross_entropy is to the
     mean loss: bf16 tensor-core products (operands in fp32 are rounded, as there), but the logits stay unrounded fp32 sums and are
     never in memory; a forward that waits for its backward holds N * V 16-bit values.  Negative tokens and those >= V as in
-    token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold, and takes no time in the
-    products (the rows that name a token are listed on the device).  A tangent is refused."""
+    token_logprobs: a left-out row has 0 and 0 and no part in the gradients, whatever its activations hold, and is in none of the
+    products (the rows that name a token are listed on the device; the list, its copy and the activations' gradient go over all).  A tangent is refused."""
     if weight.dim() != 2 or act.dim() < 1 or act.shape[-1] != weight.shape[1]:
         raise ValueError(f"hawk_b200: activations of shape {tuple(act.shape)} with a weight of shape {tuple(weight.shape)}")
     want = torch.is_grad_enabled() and (weight.requires_grad or act.requires_grad)

@@ -388,10 +388,10 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constan
         const long long label = score_label;
         // In a row whose token is all but certain the other elements are what 1 - p is made of, and lost beside its 1.  Where the
         // odd and the even columns' maxima lie so far apart that the others may be little, the elements at the maximum are kept apart
-        // from the sum, and counted; where they do not, the others are 2^-9 at least, and right to 2^-14 within the sum.  Scores of 1238 rows of
+        // from the sum, and counted; where they do not, the others are 2^-9 at least, and right to 2^-13 within the sum.  Scores of 1238 rows of
         // H512 V32000 with e kept, most of their tokens likely: 50.2 us without this, 53.6 with, 54.7 with four chunks unrolled here too;
         // a check of every chunk, or of the chunk at the maximum only, 59.5; of unlikely tokens, and at H2048, 0.1 to 0.7 % more.
-        const bool lone = fabsf(m0 - m1) > 6.25f;
+        const bool lone = fabsf(m0 - m1) > 6.2f;  // e^-6.2 is a little more than 2^-9
         float2 s = f2(0.f), sx = f2(0.f), rest = f2(0.f);
         const auto sums = [&](auto with) {
         constexpr bool APART = decltype(with)::value;

@@ -215,14 +215,14 @@ class Embedding(nn.Embedding):
         super().__init__(*args, **kwargs)
         self.scale = scale
 
-    def forward(self, ids):
+    def forward(self, input):
         w = self.weight
         if (not w.is_cuda or w.dtype not in (torch.float32, torch.bfloat16) or self.max_norm is not None or self.scale_grad_by_freq
-                or self.sparse or type(w) not in (torch.Tensor, nn.Parameter) or type(ids) is not torch.Tensor
+                or self.sparse or type(w) not in (torch.Tensor, nn.Parameter) or type(input) is not torch.Tensor
                 or (not torch.compiler.is_compiling() and ops._transformed())):
-            out = super().forward(ids)
+            out = super().forward(input)
             return out if self.scale == 1.0 else out * self.scale
-        return ops.embedding(ids, w, self.scale, self.padding_idx)
+        return ops.embedding(input, w, self.scale, self.padding_idx)
 
 
 class MLP(nn.Module):

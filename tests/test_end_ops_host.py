@@ -163,3 +163,13 @@ def test_operators_without_a_forward_derivative_refuse_tangents(way):
         assert torch.equal(op(x), 2 * x)  # no tangent
     assert all(o.reverse_only for o in (ops.embedding_fwd, ops.embedding_bwd, ops.token_logprobs_fwd, ops.token_logprobs_bwd,
                                         ops.linear_logprobs_fwd, ops.linear_logprobs_bwd))
+
+
+def test_embedding_takes_its_argument_by_name():
+    """The model's table is called as nn.Embedding is."""
+    import inspect
+
+    import hawk_b200.model as M
+    e, ids = M.HawkModel(M.HawkConfig(96, 64, 128, 1, 64, 4, 4)).embed_tokens, torch.tensor([3, 95])
+    assert torch.equal(e(input=ids), e.weight[ids])
+    assert inspect.signature(type(e).forward).parameters.keys() == inspect.signature(torch.nn.Embedding.forward).parameters.keys()

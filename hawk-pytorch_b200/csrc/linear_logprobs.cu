@@ -12,8 +12,9 @@
 //   2. reduce  a warp per row over its groups: m, log s, log probability and entropy.  The token's own logit is formed once more,
 //      as a plain fp32 dot product: the tensor core truncates its running sum at every step of 16 products, which leaves a large
 //      logit a little too small (2e-5 of 16 after 2048 products), and a log probability near 0 would be nothing but that.  The
-//      sums get its term anew as well.  Elements at a group's maximum are counted apart where little else is in their chunk, and
-//      log s is log1p of the rest, so that 1 - p of a token that is all but certain is as exact as the logits.  N rows of act and weight read: 50 us of 11 ms at N32760 H2048 V32000.
+//      sums get its term anew as well.  Elements at a group's maximum are counted apart where little else may be in the group, and
+//      log s is log1p of the rest, so that 1 - p of a token that is all but certain is as exact as the logits.  N rows of act and
+//      weight read: 67 us of 11 ms at N32760 H2048 V32000.
 // Backward, from e and the groups' maxima (2 N V bytes kept instead of a third GEMM: forming the logits again takes 2 N H V
 // flops, 3.1 ms at N32760 H2048 V32000 where writing and reading e takes 1):
 //   3. d x     d x_j = -p_j (g_lp + g_H (log p_j + H)) with p_j = e_j e^(m_g - m - log s), and at the token from its exact log
@@ -28,9 +29,9 @@
 //      rows d W takes twice, as two bf16 numbers to each of fp32, from a scale within 2^-8 of 1 (kTwiceRows).
 //   4. two GEMMs, d act = dx W and d W = dx^T act; d act's rows go back to their places.
 // Bound by the tensor pipe: 2 N H V flops forward, 4 N H V backward.  Measured at N32760 H2048 V32000 in bf16, all rows named:
-// 3.19 ms without and 3.31 ms with what a backward needs (1.35 / 1.30 PFLOP/s), backward 6.3 ms (1.36; dx 0.7 at 5.9 TB/s, the
+// 3.13 ms without and 3.28 ms with what a backward needs (1.37 / 1.31 PFLOP/s), backward 6.2 to 6.5 ms (1.34; dx 0.7, the
 // GEMMs 2.74 and 2.80), 10.3 ms together in a sustained loop with a tenth left out.  At small H the logits' epilogue sets the pace:
-// H512 N3108 118 us without, 136 with (0.06 of MMAs).
+// H512 N3108 110 us without, 132 with (0.06 of MMAs).
 #include "head_gemm.cuh"
 
 namespace hawk {
